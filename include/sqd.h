@@ -760,6 +760,69 @@ int sqd_comm_allreduce(sqd_comm *comm, void *buf, int64_t count, int dtype, int 
 int sqd_comm_broadcast(sqd_comm *comm, void *buf, int64_t count, int dtype, int root, void *stream);
 int sqd_comm_destroy(sqd_comm *comm);
 
+/* ------------------------------------------------------------------------------------------------
+ * Token operators of image / video encoders: (20) residual RMS norm, (21) rotary positions over several axes, (22) attention.
+ * Element types: SQD_F32 | SQD_BF16 | SQD_F16 (a `dtype` argument); sums, softmax statistics, angles and gradients' accumulators are
+ * fp32 or wider, outputs are rounded once.  Deterministic: no atomics.  No workspace is kept between calls, so captured graphs that
+ * own their buffers do not share any.                                                                                             */
+#define SQD_F32 0
+#define SQD_BF16 1
+#define SQD_F16 2
+
+/* (20) rows [rows, C], dense.  stream_out = round(x + res) (NULL with res NULL: the rows themselves are normalised),
+ * y = w * s / sqrt(mean(s^2) + eps) with s = the ROUNDED stream; rstd [rows] (or NULL) is what the backward reads.  w [C] in the rows'
+ * type or fp32 (wdtype).
+ * bwd: gy, gs (gradient that arrives at the stream, or NULL) -> gx [rows, C] (the gradient of x and of res alike), gw [C] in w's type;
+ * part: sqd_rms_norm_nblk(rows) x C floats of scratch.                                                                              */
+int sqd_rms_norm_fwd(const void *x, const void *res, const void *w, void *y, void *stream_out, float *rstd, int64_t rows, int C, float eps,
+                     int dtype, int wdtype, void *stream);
+int sqd_rms_norm_nblk(int64_t rows);
+int sqd_rms_norm_bwd(const void *gy, const void *gs, const void *s, const void *w, const float *rstd, void *gx, void *gw, float *part,
+                     int64_t rows, int C, int dtype, int wdtype, void *stream);
+
+/* (21) q [B,S,Hq,D], k [B,S,Hk,D] (Hk = 0: queries alone) with element strides of batch, token and head, features dense -> dense q_out,
+ * k_out.  pos [S,axes] (pos_batch_stride 0) or [B,S,axes], int32 or int64 (pos_bytes); pairs[a]: how many of the P = sum(pairs) <= D/2
+ * pairs turn with axis a, in order; freq [P] fp64, radians per unit of position.  Pairs are (p, p+P), interleaved: (2p, 2p+1); the
+ * features behind 2P pass unchanged.  inverse: by the negative angle (the backward).                                                */
+typedef struct sqd_rotary_args {
+    const void *q, *k;
+    void *q_out, *k_out;
+    const void *pos;
+    const double *freq;
+    void *stream;
+    int64_t q_stride[3], k_stride[3], pos_batch_stride;
+    int32_t pairs[4];
+    int32_t B, S, Hq, Hk, D, axes, pos_bytes, interleaved, inverse, dtype;
+} sqd_rotary_args;
+int sqd_rotary_axes(const sqd_rotary_args *a);
+
+/* (22) attention.  q [B,Sq,Hq,D]; k, v [B,Sk,Hkv,D], Hq a multiple of Hkv (head h reads key head h / (Hq/Hkv)); element strides of batch,
+ * token, head; features dense; pointers and strides 16-byte aligned; D a multiple of 8 up to 128.
+ *   z = scale q.k;  softcap c > 0: z = c tanh(z / c);  slopes [Hq] (or NULL): z -= slope |pos_i - j|
+ *   pos_i = i + n - Sq, n = k_len[b] (or NULL: Sk): the queries are the LAST Sq of n positions.  Keys j >= n are hidden.
+ *   causal: j <= pos_i is seen; prefix [B] (or NULL; causal only): j < prefix[b] too
+ *   q_docs [B,Sq], k_docs [B,Sk] (both or neither): i sees j where the two are equal and >= 0 (negative: padding)
+ * A row that sees no key gets zeros.  Keys that no query may see (j >= n, negative document) are read as zeros, whatever they hold.
+ *   fwd: o [B,Sq,Hq,D] dense; lse [B,Hkv,Sq*G] (G = Hq/Hkv, row i*G + g; log2 of the softmax sum in base-2 scores, +inf for an empty row)
+ *        or NULL.  scratch: sqd_attn_fwd_scratch(a) floats (keys split over workgroups when there are few rows; 0: none needed).
+ *   bwd: q, k, v, o, lse as of the forward, go [B,Sq,Hq,D] with its own strides -> gq [B,Sq,Hq,D], gk, gv [B,Sk,Hkv,D] dense;
+ *        scratch: sqd_attn_bwd_scratch(a) floats.                                                                                    */
+typedef struct sqd_attn_args {
+    const void *q, *k, *v, *go;
+    void *o, *gq, *gk, *gv;
+    float *lse, *scratch;
+    const float *slopes;
+    const int32_t *prefix, *q_docs, *k_docs, *k_len;
+    void *stream;
+    int64_t q_stride[3], k_stride[3], v_stride[3], go_stride[3];
+    float scale, softcap;
+    int32_t B, Sq, Sk, Hq, Hkv, D, causal, dtype;
+} sqd_attn_args;
+int64_t sqd_attn_fwd_scratch(const sqd_attn_args *a);
+int sqd_attn_fwd(const sqd_attn_args *a);
+int64_t sqd_attn_bwd_scratch(const sqd_attn_args *a);
+int sqd_attn_bwd(const sqd_attn_args *a);
+
 #ifdef __cplusplus
 }
 #endif

@@ -290,6 +290,14 @@ _SIGNATURES = {
     "sqd_smooth_nblk": (_I, [_I, _I]),
     "sqd_smooth_fwd": (_I, [_P, _P, _P, _I, _P, _I, _I, _I, _P]),
     "sqd_smooth_bwd": (_I, [_P, _P, _P, _I, _P, _F, _P, ctypes.c_int64, _I, _I, _I, _P]),
+    "sqd_rms_norm_fwd": (_I, [_P] * 6 + [ctypes.c_int64, _I, _F, _I, _I, _P]),
+    "sqd_rms_norm_nblk": (_I, [ctypes.c_int64]),
+    "sqd_rms_norm_bwd": (_I, [_P] * 8 + [ctypes.c_int64, _I, _I, _I, _P]),
+    "sqd_rotary_axes": (_I, [_P]),
+    "sqd_attn_fwd_scratch": (ctypes.c_int64, [_P]),
+    "sqd_attn_fwd": (_I, [_P]),
+    "sqd_attn_bwd_scratch": (ctypes.c_int64, [_P]),
+    "sqd_attn_bwd": (_I, [_P]),
     "sqd_chain_loss": (_I, [_P, _I, _P, _I, ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float, _P, _P]),
 }
 

@@ -17,6 +17,7 @@ BACKEND = {
     "pose_head": "hip", "depthwise_conv": "hip", "squeeze_excite": "hip", "linear": "hip (1x1 implicit GEMM over rows)",
     "transformer_encoder": "hip (fused attention up to 512 tokens — 256 at embedding width 56 / 64 —, feed-forward, add+dropout+layernorm)",
     "full_query_layer": "hip", "bins_head": "hip",
+    "rms_norm_residual": "hip", "rotary_axes": "hip", "attention": "hip (fp32 / bf16 / fp16, heads of up to 128 features)",
 }
 
 ATEN_CALLS = {}               # operator -> calls that ran on ATen: nothing writes to it any more (kept so that tests can assert it stays empty)
@@ -332,3 +333,138 @@ def bins_head(energy_maps, conv1x1, y, min_val, max_val, raw_linear=False):
     if not ops.bins_supported(Q, D):
         raise RuntimeError("sqd: bins head kernel supports Q, dim_out <= 128; got Q=%d dim_out=%d" % (Q, D))
     return ops.BinsHead.apply(energy_maps, conv1x1.weight, conv1x1.bias, centers)
+
+
+# ---- token operators of image / video encoders (csrc/token_norm.hip, rotary.hip, attention*.hip) --------------------------------------
+def _token_tensor(who, name, t, dim, like=None):
+    """the checks that every tensor of a token operator passes; `like`: same element type and device"""
+    from . import tokens
+    if not isinstance(t, torch.Tensor) or t.dim() != dim:
+        raise RuntimeError("sqd: %s: %s must be a tensor of %d dimensions" % (who, name, dim))
+    if not t.is_cuda:
+        raise RuntimeError("sqd: %s must run on the MI355X (HIP) device: %s is on %s; there is no CPU fallback" % (who, name, t.device))
+    if t.dtype not in tokens.DTYPE:
+        raise RuntimeError("sqd: %s: %s is %s (float32, bfloat16 or float16)" % (who, name, t.dtype))
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise RuntimeError("sqd: %s: %s is %s on %s, the first tensor %s on %s" % (who, name, t.dtype, t.device, like.dtype, like.device))
+
+
+def _index_tensor(who, name, t, shape, device, types):
+    if not isinstance(t, torch.Tensor) or t.dtype not in types or t.device != device or tuple(t.shape) != tuple(shape):
+        raise RuntimeError("sqd: %s: %s must be %s of shape %s on %s" % (who, name, " | ".join(str(d) for d in types), tuple(shape), device))
+    return t.contiguous()
+
+
+def rms_norm_residual(x, weight, residual=None, eps=1e-6):
+    """stream = x + residual, kept in the rows' type; y = weight * stream / sqrt(mean(stream^2) + eps) over the last dimension.
+    x, residual [..., C] (float32 | bfloat16 | float16), weight [C] in that type or float32 -> (y, stream); residual None: (y, x).
+    Differentiable in x, residual (the gradients of both outputs join) and weight."""
+    who = "rms_norm_residual"
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise RuntimeError("sqd: %s: x must be a tensor [..., C]" % who)
+    _token_tensor(who, "x", x, x.dim())
+    C = x.shape[-1]
+    _token_tensor(who, "weight", weight, 1)
+    if C < 1 or weight.shape[0] != C or weight.device != x.device or weight.dtype not in (x.dtype, torch.float32):
+        raise RuntimeError("sqd: %s: weight %s %s on %s against rows of %d features in %s" % (who, tuple(weight.shape), weight.dtype, weight.device, C, x.dtype))
+    if residual is not None:
+        _token_tensor(who, "residual", residual, x.dim(), x)
+        if residual.shape != x.shape:
+            raise RuntimeError("sqd: %s: residual %s against x %s" % (who, tuple(residual.shape), tuple(x.shape)))
+    if not eps >= 0.0:
+        raise RuntimeError("sqd: %s: eps = %r" % (who, eps))
+    from . import tokens
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        out = tokens.RmsNormResidual.apply(x, weight, residual, float(eps))
+        return out if residual is not None else (out, x)
+    with tokens.on_device(x):
+        y, s, _ = tokens._norm_fwd(x, weight.contiguous(), residual, float(eps), False)
+    return (y, s) if residual is not None else (y, x)
+
+
+def rotary_frequencies(pairs, theta=10000.0, shared=False, device="cuda"):
+    """The frequency table [sum(pairs)] (float64, radians per unit of position) of rotary_axes.  Every axis a has its own ladder
+    theta^(-t / pairs[a]), t = 0 .. pairs[a] - 1; shared: one ladder theta^(-p / sum(pairs)) runs through the axes."""
+    n = sum(pairs)
+    if shared:
+        e = torch.arange(n, dtype=torch.float64) / max(1, n)
+    else:
+        e = torch.cat([torch.arange(p, dtype=torch.float64) / max(1, p) for p in pairs])
+    return (float(theta) ** (-e)).to(device)
+
+
+def rotary_axes(q, k, positions, freq, pairs, interleaved=False):
+    """Rotary positions over 1 to 4 axes (time, row, column).  q [B,S,Hq,D], k [B,S,Hk,D] or None; positions [S,A] or [B,S,A] (int32 | int64, any
+    sign and size); pairs: for each axis how many of the head's rotation pairs turn with it, P = sum(pairs) <= D / 2 in order; freq [P] float64
+    (rotary_frequencies).  Pair p is (p, p + P), interleaved: (2p, 2p + 1); features behind 2P pass unchanged.  -> new dense q, k.
+    Angles are taken in 64 bits.  Differentiable in q and k."""
+    who = "rotary_axes"
+    _token_tensor(who, "q", q, 4)
+    B, S, Hq, D = q.shape
+    if k is not None:
+        _token_tensor(who, "k", k, 4, q)
+        if k.shape[:2] != q.shape[:2] or k.shape[3] != D:
+            raise RuntimeError("sqd: %s: k %s against q %s" % (who, tuple(k.shape), tuple(q.shape)))
+    pairs = tuple(int(p) for p in pairs)
+    P = sum(pairs)
+    if not 1 <= len(pairs) <= 4 or min(pairs) < 0 or P < 1 or 2 * P > D or D % 2 or D > 1024:
+        raise RuntimeError("sqd: %s: rotation pairs %s in heads of %d features (1 to 4 axes, an even number of features up to 1024)" % (who, pairs, D))
+    if not isinstance(positions, torch.Tensor) or positions.dim() not in (2, 3):
+        raise RuntimeError("sqd: %s: positions must be [S,A] or [B,S,A]" % who)
+    positions = _index_tensor(who, "positions", positions, ((S,) if positions.dim() == 2 else (B, S)) + (len(pairs),), q.device, (torch.int32, torch.int64))
+    freq = _index_tensor(who, "freq", freq, (P,), q.device, (torch.float64,))
+    from . import tokens
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = tokens.RotaryAxes.apply(q, k, positions, freq, pairs, int(bool(interleaved)))
+        return out if k is not None else (out, None)
+    return tokens._rotate(q, k, positions, freq, pairs, int(bool(interleaved)), 0)
+
+
+def attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefix=None, q_docs=None, k_docs=None, k_len=None):
+    """softmax(z) v over the keys a query may see.  q [B,Sq,Hq,D]; k, v [B,Sk,Hkv,D], Hq a multiple of Hkv; D a multiple of 8 up to 128; float32 |
+    bfloat16 | float16; any strides.  -> o [B,Sq,Hq,D].
+
+    z = scale q.k (scale > 0, default 1 / sqrt(D)); softcap c > 0: z = c tanh(z / c); slopes [Hq] float32: z -= slope |pos_i - j|.
+    The queries are the last Sq positions of a row's n keys: pos_i = i + n - Sq with n = k_len[b] (int32 [B], default Sk; a cache longer
+    than its contents), keys from n on are hidden.  causal: query i sees j <= pos_i, and j < prefix[b] (int32 [B]) whatever its own position.
+    q_docs [B,Sq], k_docs [B,Sk] (int32; k_docs defaults to q_docs where Sq = Sk): i sees j of its own document; a negative document is padding.
+
+    A query that sees no key gets zeros, and zero gradients.  Keys behind n, padding keys and padding queries may hold anything.  Elsewhere a
+    masked product is zero times the value, as in any matrix product: an infinite or NaN value that SOME query of the call sees may reach
+    others.  Differentiable in q, k, v; slopes are constants (refused if they require a gradient)."""
+    who = "attention"
+    _token_tensor(who, "q", q, 4), _token_tensor(who, "k", k, 4, q), _token_tensor(who, "v", v, 4, q)
+    B, Sq, Hq, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise RuntimeError("sqd: %s: q %s, k %s, v %s" % (who, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if D % 8 or not 8 <= D <= 128:
+        raise RuntimeError("sqd: %s: heads of %d features: the kernel takes multiples of 8 up to 128" % (who, D))
+    scale = float(scale) if scale is not None else D ** -0.5
+    softcap = float(softcap or 0.0)
+    if not 0.0 < scale < 3e38 or not 0.0 <= softcap < 3e38:
+        raise RuntimeError("sqd: %s: scale %r must be positive, softcap %r not negative" % (who, scale, softcap))
+    if slopes is not None:
+        if slopes.requires_grad:
+            raise RuntimeError("sqd: %s: the slopes of the distance bias are constants; no gradient is computed for them" % who)
+        slopes = _index_tensor(who, "slopes", slopes, (Hq,), q.device, (torch.float32,))
+    i32 = (torch.int32,)
+    if prefix is not None:
+        if not causal:
+            raise RuntimeError("sqd: %s: a prefix needs causal=True" % who)
+        prefix = _index_tensor(who, "prefix", prefix, (B,), q.device, i32)
+    if k_docs is None and q_docs is not None and Sq == Sk:
+        k_docs = q_docs
+    if (q_docs is None) != (k_docs is None):
+        raise RuntimeError("sqd: %s: documents of queries and keys come together" % who)
+    if q_docs is not None:
+        q_docs = _index_tensor(who, "q_docs", q_docs, (B, Sq), q.device, i32)
+        k_docs = _index_tensor(who, "k_docs", k_docs, (B, Sk), q.device, i32)
+    if k_len is not None:
+        k_len = _index_tensor(who, "k_len", k_len, (B,), q.device, i32)
+    from . import tokens
+    cfg, masks = (scale, softcap, int(bool(causal))), (slopes, prefix, q_docs, k_docs, k_len)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return tokens.Attention.apply(q, k, v, cfg, *masks)
+    with tokens.on_device(q):
+        return tokens.attn_fwd(tokens._rows16(q), tokens._rows16(k), tokens._rows16(v), cfg, masks, False)[0]
