@@ -804,12 +804,12 @@ int sqd_rotary_axes(const sqd_rotary_args *a);
  *   q_docs [B,Sq], k_docs [B,Sk] (both or neither): i sees j where the two are equal and >= 0 (negative: padding)
  * A row that sees no key gets zeros.  Keys that no query may see (j >= n, negative document) are read as zeros, whatever they hold.
  *   fwd: o [B,Sq,Hq,D] dense; lse [B,Hkv,Sq*G] (G = Hq/Hkv, row i*G + g; log2 of the softmax sum in base-2 scores, +inf for an empty row)
- *        or NULL.  scratch: sqd_attn_fwd_scratch(a) floats (keys split over workgroups when there are few rows; 0: none needed).
- *   bwd: q, k, v, o, lse as of the forward, go [B,Sq,Hq,D] with its own strides -> gq [B,Sq,Hq,D], gk, gv [B,Sk,Hkv,D] dense;
+ *        or NULL; o_low (16-bit types, or NULL): what o's rounding left, for the backward.  scratch: sqd_attn_fwd_scratch(a) floats (keys split over workgroups when there are few rows; 0: none needed).
+ *   bwd: q, k, v, o, o_low (or NULL: gradients lose a little), lse as of the forward, go [B,Sq,Hq,D] with its own strides -> gq [B,Sq,Hq,D], gk, gv [B,Sk,Hkv,D] dense;
  *        scratch: sqd_attn_bwd_scratch(a) floats.                                                                                    */
 typedef struct sqd_attn_args {
     const void *q, *k, *v, *go;
-    void *o, *gq, *gk, *gv;
+    void *o, *o_low, *gq, *gk, *gv;
     float *lse, *scratch;
     const float *slopes;
     const int32_t *prefix, *q_docs, *k_docs, *k_len;

@@ -22,13 +22,14 @@ namespace sqd {
 
 struct AttnK {
     const void *q, *k, *v, *go;
-    void *o, *gq, *gk, *gv;
+    void *o, *o_low, *gq, *gk, *gv;
     float *lse, *delta, *part_o, *part_lse;
     const float *slopes;
     const int *prefix, *q_docs, *k_docs, *k_len;
     const int2 *doc_rng;                    // per tile of the looped-over side: smallest and largest document id
     int64_t qs[3], ks[3], vs[3], gos[3];
-    float scale_log2, cap_in, cap_out, cap_grad, scale;   // see Score
+    float scale_log2, cap_in, cap_out, scale;             // log2(e) scale; 2 log2(e) scale / cap, cap log2(e)
+    unsigned g_magic;
     int B, Sq, Sk, Hq, Hkv, G, D, causal, ntile, nsplit, ndoc_tiles;
 };
 
@@ -130,30 +131,81 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// a ROWS x DP tile on its way from memory to LDS by NTH threads: 16-byte pieces in registers between load() and store()
+// 16 bytes of this lane's address to LDS byte `lds` + 16 * lane, without a register in between.  The compiler does not see the load: dma_wait()
+// (and a barrier, for other waves' data) comes before the LDS bytes are read.  Lanes switched off leave their 16 bytes as they are.
+__device__ __forceinline__ void dma16(const void *g, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_offset(const void *p) {
+    return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)p);
+}
+
+// a ROWS x DP tile from memory to LDS by NTH threads.  The LDS side of a DMA is linear in the lane, so the permutation of the pieces is applied to
+// the address a lane reads.  Pieces that are not loaded (rows nobody may see, features past D) keep what the buffer held: zeros at the start
+// (clear()), later an older tile's rows, which are data of this call: finite wherever the inputs that count are.
 template <typename T, int DP, int ROWS, int NTH> struct Stage {
     typedef Tile<T, DP> L;
-    static constexpr int TOTAL = ROWS * L::CH, N = (TOTAL + NTH - 1) / NTH;
-    u32x4 reg[N];
-    // row_at(r): pointer to row r of the tile, or nullptr (zeros)
-    template <typename F> __device__ __forceinline__ void load(int tid, int D, F &&row_at) {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int idx = tid + n * NTH, r = idx / L::CH, c = idx % L::CH;
-            u32x4 w = {0, 0, 0, 0};
-            const T *p = idx < TOTAL ? row_at(r) : nullptr;
-            if (p && c * L::CHE < D) w = *reinterpret_cast<const u32x4 *>(p + c * L::CHE);
-            reg[n] = w;
-        }
-    }
-    __device__ __forceinline__ void store(char *t, int tid) {
+    static constexpr int TOTAL = ROWS * L::CH, N = (TOTAL + NTH - 1) / NTH, BYTES = ROWS * L::PITCH;
+    int row[N], col[N];                     // this thread's pieces: tile row, first feature
+    __device__ __forceinline__ Stage(int tid) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int idx = tid + n * NTH;
-            if (idx < TOTAL) *reinterpret_cast<u32x4 *>(t + L::at(idx / L::CH, idx % L::CH)) = reg[n];
+            row[n] = idx < TOTAL ? idx / L::CH : -1;
+            col[n] = ((idx % L::CH) ^ (bitrev4((idx / L::CH) & 15) & L::ROT)) * L::CHE;
+        }
+    }
+    // row_at(n, r): the address of tile row r = row[n], or nullptr
+    template <typename F> __device__ __forceinline__ void load(unsigned lds, int tid, int D, F &&row_at) {
+        const unsigned wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (row[n] < 0) continue;
+            const T *p = row_at(n, row[n]);
+            if (p && col[n] < D) dma16(p + col[n], lds + (wave * 64 + n * NTH) * 16);
         }
     }
 };
+
+// zeros over `bytes` (a multiple of 16) of LDS by NTH threads
+template <int NTH> __device__ __forceinline__ void clear_lds(char *p, int bytes, int tid) {
+    for (int i = tid * 16; i < bytes; i += NTH * 16) *reinterpret_cast<u32x4 *>(p + i) = u32x4{0, 0, 0, 0};
+}
+
+// the tiles of [.., end) whose documents meet [lo, hi]: 64 tiles' ranges are looked at together, one a lane, and kept as two masks
+struct DocWalk {
+    const int2 *rng;                        // nullptr: every tile
+    int lo, hi, end, base;
+    unsigned long long see, uni;
+    __device__ __forceinline__ DocWalk(const int2 *r, int lo_, int hi_, int end_) : rng(r), lo(lo_), hi(hi_), end(end_), base(-64), see(0), uni(0) {}
+    // first tile >= t, `end` if none; one_doc: the tile and [lo, hi] are one and the same document
+    __device__ __forceinline__ int next(int t, bool &one_doc) {
+        one_doc = true;
+        if (!rng) return min(t, end);
+        while (t < end) {
+            if (t - base >= 64) {
+                base = t & ~63;
+                const int u = base + (int)__lane_id();
+                int2 r = make_int2(0x7fffffff, -1);
+                if (u < end) r = rng[u];
+                see = __ballot(r.y >= lo && r.x <= hi);
+                uni = __ballot(lo == hi && r.x == lo && r.y == lo);
+            }
+            const unsigned long long m = see >> (t - base);
+            if (m) {
+                t += __builtin_ctzll(m);
+                one_doc = (uni >> (t - base)) & 1;
+                return t;
+            }
+            t = base + 64;
+        }
+        return end;
+    }
+};
+
+// R / G by a multiplication (R G < 2^32, checked on the host); magic = ceil(2^32 / G), 0 for G = 1
+__device__ __forceinline__ int div_g(int R, unsigned magic) { return magic ? (int)__umulhi((unsigned)R, magic) : R; }
 
 // the larger / sum of the two half-waves' values, in both halves
 __device__ __forceinline__ float half_max(float v) {
@@ -175,6 +227,24 @@ template <bool CAP> __device__ __forceinline__ float tanh_of(float raw, float ca
 
 // what a row may see: keys j <= lim (lengths, causal order and prefix in one number), document equal
 __device__ __forceinline__ int row_limit(int pos, int len, bool causal, int prefix) { return causal ? min(max(pos, prefix - 1), len - 1) : len - 1; }
+
+// what one lane knows of its row
+struct RowOf {
+    int i, g, pos, qd, lim;
+    bool on;
+};
+__device__ __forceinline__ RowOf row_of(const AttnK &A, int b, int R, int RT, int len, int prefix) {
+    RowOf r;
+    r.on = R < RT;
+    r.i = r.on ? div_g(R, A.g_magic) : A.Sq - 1;
+    r.g = r.on ? R - r.i * A.G : 0;
+    r.pos = r.i + len - A.Sq;
+    r.qd = -2;
+    if (A.q_docs && r.on) r.qd = max(A.q_docs[(int64_t)b * A.Sq + r.i], -1);
+    if (r.qd == -1) r.qd = -2;
+    r.lim = r.on && (!A.q_docs || r.qd >= 0) ? row_limit(r.pos, len, A.causal, prefix) : -1;
+    return r;
+}
 
 // n workgroups dealt to 8 XCDs round robin: workgroup id -> work item such that an XCD gets consecutive items (they share keys and values in
 // its L2)

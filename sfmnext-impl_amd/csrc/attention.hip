@@ -26,112 +26,31 @@ __global__ __launch_bounds__(64) void doc_range_kernel(const int *__restrict__ i
     if (threadIdx.x == 0) out[(int64_t)b * ntile + t] = make_int2(lo, hi);
 }
 
-template <typename T, int DP, int KT, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_fwd_kernel(AttnK A) {
+// four neighbouring features of the output, and what their rounding left (o_low: the backward's delta wants o to more bits than o has)
+template <typename T> __device__ __forceinline__ void store_out(const AttnK &A, int64_t at, const float (&v)[4]) {
+    store_f32<T, 4>((T *)A.o + at, v);
+    if (sizeof(T) == 2 && A.o_low) {
+        float r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = v[e] - to_f32(from_f32<T>(v[e]));
+        store_f32<T, 4>((T *)A.o_low + at, r);
+    }
+}
+
+// The scores of one tile (x: raw products, NB blocks of 32 keys by the wave's 32 rows), the running maximum and sum, and the second product.
+template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
     typedef Tile<T, DP> L;
-    typedef typename L::frag frag;
-    constexpr int NB = KT / 32, DB = DP / 32;
-    __shared__ __align__(16) char lk[2][KT * L::PITCH], lv[2][KT * L::PITCH];
-    __shared__ __align__(16) int ld[2][KT];
-    __shared__ int wq[8];
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    int w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = A.ntile - 1 - w % A.ntile;                 // the longest causal rows first
-    w /= A.ntile;
-    const int split = w % A.nsplit, bh = w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
-    const int RT = A.Sq * A.G, row0 = tile * BM;
-    const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk, off = len - A.Sq;
-    const int prefix = A.prefix ? A.prefix[b] : 0;
-
-    // this lane's row (both half-waves hold the same 32 rows)
-    const int R = row0 + wave * 32 + (lane & 31);
-    const bool on = R < RT;
-    const int i = on ? R / A.G : A.Sq - 1, g = on ? R - i * A.G : 0, pos = i + off;
-    int qd = -2;
-    if (A.q_docs && on) {
-        qd = A.q_docs[(int64_t)b * A.Sq + i];
-        if (qd < 0) qd = -2;
-    }
-    const int lim = on && qd != -2 || (on && !A.q_docs) ? row_limit(pos, len, A.causal, prefix) : -1;
-
-    // keys any row of the workgroup may see
-    int kend = len;
-    if (A.causal) kend = max(0, min(len, max(min(A.Sq - 1, (row0 + BM - 1) / A.G) + off + 1, prefix)));
-    int dlo = 0x7fffffff, dhi = -1;
-    if (A.q_docs) {
-        int lo = qd >= 0 ? qd : 0x7fffffff, hi = qd;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            lo = min(lo, __shfl_xor(lo, o, 64));
-            hi = max(hi, __shfl_xor(hi, o, 64));
-        }
-        if (lane == 0) wq[wave] = lo, wq[4 + wave] = hi;
-        __syncthreads();
-        dlo = min(min(wq[0], wq[1]), min(wq[2], wq[3]));
-        dhi = max(max(wq[4], wq[5]), max(wq[6], wq[7]));
-    }
-    const int nt_all = (kend + KT - 1) / KT, per = (nt_all + A.nsplit - 1) / A.nsplit;
-    const int t0 = min(nt_all, split * per), t1 = min(nt_all, t0 + per);
-    const int2 *rng = A.doc_rng + (int64_t)b * A.ndoc_tiles;
-    auto next = [&](int t) {
-        if (A.q_docs)
-            while (t < t1 && (rng[t].y < dlo || rng[t].x > dhi)) ++t;
-        return t;
-    };
-
-    frag qf[L::KS];
-    const T *qrow = (const T *)A.q + b * A.qs[0] + (int64_t)i * A.qs[1] + (int64_t)(hk * A.G + g) * A.qs[2];
-#pragma unroll
-    for (int ks = 0; ks < L::KS; ++ks) qf[ks] = L::mem_frag(qrow, ks, h, A.D, on);
-
-    const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
-    const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
-    Stage<T, DP, KT, NT> sk, sv;
-    int sd = -1;
-    auto fetch = [&](int t) {
-        const int j0 = t * KT;
-        auto row_of = [&](const T *base, int64_t stride) {
-            return [=](int r) -> const T * {
-                const int j = j0 + r;
-                if (j >= len || (kdoc && kdoc[j] < 0)) return nullptr;
-                return base + j * stride;
-            };
-        };
-        sk.load(tid, A.D, row_of(kbase, A.ks[1]));
-        sv.load(tid, A.D, row_of(vbase, A.vs[1]));
-        if (kdoc && tid < KT) sd = j0 + tid < len ? kdoc[j0 + tid] : -1;
-    };
-    auto put = [&](int s) {
-        sk.store(lk[s], tid);
-        sv.store(lv[s], tid);
-        if (kdoc && tid < KT) ld[s][tid] = sd;
-    };
-
-    const float slope = BIAS && on ? A.slopes[hk * A.G + g] * 1.44269504088896341f : 0.f;
+    static constexpr int DB = DP / 32;
     f32x16 o[DB];
+    float m, l;
+    __device__ __forceinline__ Softmax() : m(-INFINITY), l(0.f) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db) o[db] = f32x16{};
-    float m = -INFINITY, l = 0.f;
-
-    int t = next(t0), s = 0;
-    if (t < t1) {
-        fetch(t);
-        put(0);
+        for (int db = 0; db < DB; ++db) o[db] = f32x16{};
     }
-    __syncthreads();
-    while (t < t1) {
-        const int tn = next(t + 1);
-        if (tn < t1) fetch(tn);
-        const int j0 = t * KT;
-
-        f32x16 x[NB];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            x[nb] = f32x16{};
-#pragma unroll
-            for (int ks = 0; ks < L::KS; ++ks) x[nb] = Mma<T>::mma(L::row_frag(lk[s], nb * 32 + (lane & 31), ks, h), qf[ks], x[nb]);
-        }
+    // j0: first key; lim, qd: the row's limit and document; ld: the tile's documents (docs); part: some row does not see the whole tile
+    __device__ __forceinline__ void tile(f32x16 (&x)[NB], const AttnK &A, const char *lv, const int *ld, bool docs, bool part, int j0, int pos, int lim, int qd,
+                                         float slope, int lane) {
+        const int h = lane >> 5;
         if (CAP || BIAS) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -143,9 +62,6 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 }
         }
         const float c = CAP || BIAS ? 1.f : A.scale_log2;
-        // the mask, where a row of the wave does not see the whole tile
-        bool part = __any(lim < j0 + KT - 1);
-        if (kdoc) part = part || !(dlo == dhi && rng[t].x == dlo && rng[t].y == dlo);
         if (part) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -153,7 +69,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int r4 = 0; r4 < 4; ++r4) {
                     const int j4 = nb * 32 + 8 * r4 + 4 * h;
                     int4 kd = make_int4(qd, qd, qd, qd);
-                    if (kdoc) kd = *reinterpret_cast<const int4 *>(&ld[s][j4]);
+                    if (docs) kd = *reinterpret_cast<const int4 *>(ld + j4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
@@ -166,9 +82,9 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[nb][r]);
-        const float mn = fmaxf(m, half_max(mx) * c), base = mn == -INFINITY ? 0.f : mn;
-        if (__any(mn > m)) {
-            const float alpha = exp2_hw(m - base);
+        const float mn = fmaxf(m, half_max(mx) * c);
+        if (__builtin_expect(__any(mn > m), 0)) {              // rare once the maximum has settled
+            const float alpha = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
             l *= alpha;
 #pragma unroll
             for (int db = 0; db < DB; ++db)
@@ -176,32 +92,132 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
             m = mn;
         }
-        float p[NB][16];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                p[nb][r] = exp2_hw(fmaf(x[nb][r], c, -base));
-                l += p[nb][r];
-            }
-        // P is rounded to the values' type for the second product (half a step of that type, relative); the sum keeps the unrounded P
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                const frag pf = Mma<T>::pack(&p[nb][8 * kk]);
+                float p[8];
 #pragma unroll
-                for (int db = 0; db < DB; ++db) o[db] = Mma<T>::mma(L::col_frag(lv[s], nb * 32 + kk * 16, db, lane), pf, o[db]);
+                for (int r = 0; r < 8; ++r) {
+                    p[r] = exp2_hw(fmaf(x[nb][8 * kk + r], c, -base));
+                    l += p[r];
+                }
+                // P is rounded to the values' type for the second product (half a step of that type, relative); the sum keeps the unrounded P
+                const typename L::frag pf = Mma<T>::pack(p);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) o[db] = Mma<T>::mma(L::col_frag(lv, nb * 32 + kk * 16, db, lane), pf, o[db]);
             }
-        if (tn < t1) put(s ^ 1);
+    }
+};
+
+template <typename T, int DP, int KT, bool CAP, bool BIAS>
+__global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_fwd_kernel(AttnK A) {
+    typedef Tile<T, DP> L;
+    typedef typename L::frag frag;
+    typedef Stage<T, DP, KT, NT> S;
+    constexpr int NB = KT / 32, DB = DP / 32;
+    __shared__ __align__(16) char lk[2][S::BYTES], lv[2][S::BYTES];
+    __shared__ __align__(16) int ld[2][KT];
+    __shared__ int wq[8];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    int w = xcd_order(blockIdx.x, gridDim.x);
+    const int tile = A.ntile - 1 - w % A.ntile;                 // the longest causal rows first
+    w /= A.ntile;
+    const int split = w % A.nsplit, bh = w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
+    const int RT = A.Sq * A.G, row0 = tile * BM;
+    const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
+    const int prefix = A.prefix ? A.prefix[b] : 0;
+    const int R = row0 + wave * 32 + (lane & 31);               // this lane's row (both half-waves hold the same 32)
+    const RowOf row = row_of(A, b, R, RT, len, prefix);
+    clear_lds<NT>(lk[0], 2 * S::BYTES, tid);
+    clear_lds<NT>(lv[0], 2 * S::BYTES, tid);
+
+    // keys any row of the workgroup may see
+    int kend = len;
+    if (A.causal) kend = max(0, min(len, max(min(A.Sq - 1, div_g(row0 + BM - 1, A.g_magic)) + len - A.Sq + 1, prefix)));
+    int dlo = 0, dhi = 0;
+    if (A.q_docs) {
+        int lo = row.qd >= 0 ? row.qd : 0x7fffffff, hi = row.qd;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            lo = min(lo, __shfl_xor(lo, o, 64));
+            hi = max(hi, __shfl_xor(hi, o, 64));
+        }
+        if (lane == 0) wq[wave] = lo, wq[4 + wave] = hi;
+    }
+    __syncthreads();
+    if (A.q_docs) {
+        dlo = __builtin_amdgcn_readfirstlane(min(min(wq[0], wq[1]), min(wq[2], wq[3])));
+        dhi = __builtin_amdgcn_readfirstlane(max(max(wq[4], wq[5]), max(wq[6], wq[7])));
+    }
+    const int nt_all = (kend + KT - 1) / KT, per = (nt_all + A.nsplit - 1) / A.nsplit;
+    const int t0 = min(nt_all, split * per), t1 = min(nt_all, t0 + per);
+    DocWalk walk(A.q_docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, t1);
+
+    frag qf[L::KS];
+    const T *qrow = (const T *)A.q + b * A.qs[0] + (int64_t)row.i * A.qs[1] + (int64_t)(hk * A.G + row.g) * A.qs[2];
+#pragma unroll
+    for (int ks = 0; ks < L::KS; ++ks) qf[ks] = L::mem_frag(qrow, ks, h, A.D, row.on);
+
+    const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
+    const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
+    S st(tid);
+    const unsigned ok[2] = {lds_offset(lk[0]), lds_offset(lk[1])}, ov[2] = {lds_offset(lv[0]), lds_offset(lv[1])};
+    // padding keys (a negative document) are not loaded: their documents are read a tile ahead of the DMA that goes by them
+    int pd[S::N], sd = -1;
+    auto peek = [&](int t) {
+        if (!kdoc) return;
+#pragma unroll
+        for (int n = 0; n < S::N; ++n) pd[n] = t < t1 && st.row[n] >= 0 && t * KT + st.row[n] < len ? kdoc[t * KT + st.row[n]] : -1;
+        sd = t < t1 && tid < KT && t * KT + tid < len ? kdoc[t * KT + tid] : -1;
+    };
+    auto fetch = [&](int t, int s) {
+        const int j0 = t * KT;
+        auto rows = [&](const T *base, int64_t stride) {
+            const T *p0 = base + j0 * stride;
+            return [=, &pd](int n, int r) -> const T * { return j0 + r < len && (!kdoc || pd[n] >= 0) ? p0 + r * stride : nullptr; };
+        };
+        st.load(ok[s], tid, A.D, rows(kbase, A.ks[1]));
+        st.load(ov[s], tid, A.D, rows(vbase, A.vs[1]));
+        if (kdoc && tid < KT) ld[s][tid] = sd;
+    };
+
+    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * 1.44269504088896341f : 0.f;
+    Softmax<T, DP, NB, CAP, BIAS> sm;
+    int s = 0;
+    bool u, un;
+    int t = walk.next(t0, u);
+    peek(t);
+    if (t < t1) fetch(t, 0);
+    int tn = walk.next(t + 1, un);
+    peek(tn);
+    dma_wait();
+    __syncthreads();
+    while (t < t1) {
+        if (tn < t1) fetch(tn, s ^ 1);
+        bool u2 = true;
+        const int t2 = walk.next(tn + 1, u2);
+        peek(t2);
+        f32x16 x[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            x[nb] = f32x16{};
+#pragma unroll
+            for (int ks = 0; ks < L::KS; ++ks) x[nb] = Mma<T>::mma(L::row_frag(lk[s], nb * 32 + (lane & 31), ks, h), qf[ks], x[nb]);
+        }
+        // the mask, where a row of the wave does not see the whole tile
+        const bool part = !u || __any(row.lim < t * KT + KT - 1);
+        sm.tile(x, A, lv[s], ld[s], kdoc != nullptr, part, t * KT, row.pos, row.lim, row.qd, slope, lane);
+        dma_wait();
         __syncthreads();
         s ^= 1;
-        t = tn;
+        t = tn, u = un, tn = t2, un = u2;
     }
 
-    l = half_sum(l);
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    if (!on) return;
+    const float l = half_sum(sm.l), inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (!row.on) return;
     const int64_t at = (int64_t)bh * RT + R;
     if (A.nsplit > 1) {
         float *po = A.part_o + ((int64_t)split * A.B * A.Hkv * RT + at) * A.D;
@@ -210,22 +226,137 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int d = db * 32 + 8 * r4 + 4 * h;
-                const float v[4] = {o[db][4 * r4] * inv, o[db][4 * r4 + 1] * inv, o[db][4 * r4 + 2] * inv, o[db][4 * r4 + 3] * inv};
+                const float v[4] = {sm.o[db][4 * r4] * inv, sm.o[db][4 * r4 + 1] * inv, sm.o[db][4 * r4 + 2] * inv, sm.o[db][4 * r4 + 3] * inv};
                 if (d < A.D) store_f32<float, 4>(po + d, v);
             }
-        if (h == 0) A.part_lse[(int64_t)split * A.B * A.Hkv * RT + at] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+        if (h == 0) A.part_lse[(int64_t)split * A.B * A.Hkv * RT + at] = l == 0.f ? -INFINITY : sm.m + __builtin_amdgcn_logf(l);
         return;
     }
-    T *out = (T *)A.o + (((int64_t)b * A.Sq + i) * A.Hq + hk * A.G + g) * A.D;
+    const int64_t out_at = (((int64_t)b * A.Sq + row.i) * A.Hq + hk * A.G + row.g) * A.D;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
             const int d = db * 32 + 8 * r4 + 4 * h;
-            const float v[4] = {o[db][4 * r4] * inv, o[db][4 * r4 + 1] * inv, o[db][4 * r4 + 2] * inv, o[db][4 * r4 + 3] * inv};
-            if (d < A.D) store_f32<T, 4>(out + d, v);
+            const float v[4] = {sm.o[db][4 * r4] * inv, sm.o[db][4 * r4 + 1] * inv, sm.o[db][4 * r4 + 2] * inv, sm.o[db][4 * r4 + 3] * inv};
+            if (d < A.D) store_out<T>(A, out_at + d, v);
         }
-    if (A.lse && h == 0) A.lse[at] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (A.lse && h == 0) A.lse[at] = l == 0.f ? INFINITY : sm.m + __builtin_amdgcn_logf(l);
+}
+
+// Few rows (Sq G <= 32: one or some tokens against a cache).  Bandwidth bound, so what counts is bytes in flight: every wave takes 32 keys of its
+// own at a time, its K and V rows go by DMA into two private buffers, and no wave waits for another until the end, where the waves' maxima,
+// sums and outputs are joined through LDS.  Wave w of split s takes the key tiles s * per + w, + NW, ...
+template <typename T, int DP> constexpr int token_waves() { return sizeof(T) == 4 && DP == 128 ? 2 : 4; }       // 64 KB of buffers a wave in fp32
+template <typename T, int DP, int NW, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
+    typedef Tile<T, DP> L;
+    typedef typename L::frag frag;
+    typedef Stage<T, DP, 32, 64> S;
+    constexpr int DB = DP / 32;
+    static_assert(4 * S::BYTES >= 32 * DP * 4, "the buffers of a wave hold its 32 output rows in fp32");
+    __shared__ __align__(16) char buf[NW][4 * S::BYTES];        // K, V, K, V
+    __shared__ __align__(16) int ld[NW][32];
+    __shared__ float wm[NW][32], wl[NW][32];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    int w = xcd_order(blockIdx.x, gridDim.x);
+    const int split = w % A.nsplit, bh = w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
+    const int RT = A.Sq * A.G, R = lane & 31;
+    const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
+    const int prefix = A.prefix ? A.prefix[b] : 0;
+    const RowOf row = row_of(A, b, R, RT, len, prefix);
+    clear_lds<64>(buf[wave], 4 * S::BYTES, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    int kend = len;
+    if (A.causal) kend = max(0, min(len, max(len, prefix)));    // the last query sees every key
+    int dlo = row.qd >= 0 ? row.qd : 0x7fffffff, dhi = row.qd;
+    if (A.q_docs) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            dlo = min(dlo, __shfl_xor(dlo, o, 64));
+            dhi = max(dhi, __shfl_xor(dhi, o, 64));
+        }
+    }
+    const int nt_all = (kend + 31) / 32, per = ((nt_all + A.nsplit - 1) / A.nsplit + NW - 1) / NW * NW;
+    const int t0 = min(nt_all, split * per), t1 = min(nt_all, t0 + per);
+
+    frag qf[L::KS];
+    const T *qrow = (const T *)A.q + b * A.qs[0] + (int64_t)row.i * A.qs[1] + (int64_t)(hk * A.G + row.g) * A.qs[2];
+#pragma unroll
+    for (int ks = 0; ks < L::KS; ++ks) qf[ks] = L::mem_frag(qrow, ks, h, A.D, row.on);
+    const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
+    const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
+    S st(lane);
+    const unsigned o0 = lds_offset(buf[wave]);
+    auto fetch = [&](int t, int s) {
+        const int j0 = t * 32;
+        auto rows = [&](const T *base, int64_t stride) {
+            const T *p0 = base + j0 * stride;
+            return [=](int, int r) -> const T * { return j0 + r < len && (!kdoc || kdoc[j0 + r] >= 0) ? p0 + r * stride : nullptr; };
+        };
+        st.load(o0 + s * 2 * S::BYTES, lane, A.D, rows(kbase, A.ks[1]));
+        st.load(o0 + (s * 2 + 1) * S::BYTES, lane, A.D, rows(vbase, A.vs[1]));
+    };
+    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * 1.44269504088896341f : 0.f;
+    Softmax<T, DP, 1, CAP, BIAS> sm;
+    int t = t0 + wave, s = 0;
+    if (t < t1) fetch(t, 0);
+    while (t < t1) {
+        dma_wait();
+        if (t + NW < t1) fetch(t + NW, s ^ 1);
+        const int j0 = t * 32;
+        if (kdoc && lane < 32) ld[wave][lane] = j0 + lane < len ? kdoc[j0 + lane] : -1;
+        const char *lk = buf[wave] + s * 2 * S::BYTES, *lv = lk + S::BYTES;
+        f32x16 x[1] = {f32x16{}};
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ++ks) x[0] = Mma<T>::mma(L::row_frag(lk, lane & 31, ks, h), qf[ks], x[0]);
+        const bool part = kdoc != nullptr || __any(row.lim < j0 + 31);
+        sm.tile(x, A, lv, ld[wave], kdoc != nullptr, part, j0, row.pos, row.lim, row.qd, slope, lane);
+        t += NW;
+        s ^= 1;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this buffer is read before the next turn's DMA overwrites it
+    }
+    // join the waves: the row's common maximum, then the weighted sums
+    const float l = half_sum(sm.l);
+    if (h == 0) wm[wave][R] = l == 0.f ? -INFINITY : sm.m, wl[wave][R] = l;
+    __syncthreads();
+    float mx = wm[0][R];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) mx = fmaxf(mx, wm[k][R]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) sum += wl[k][R] * exp2_hw(wm[k][R] - base);
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f, mine = (l == 0.f ? 0.f : exp2_hw(sm.m - base)) * inv;
+    float *po = reinterpret_cast<float *>(buf[wave]);           // [32][DP]
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 v = {sm.o[db][4 * r4] * mine, sm.o[db][4 * r4 + 1] * mine, sm.o[db][4 * r4 + 2] * mine, sm.o[db][4 * r4 + 3] * mine};
+            *reinterpret_cast<f32x4 *>(po + R * DP + db * 32 + 8 * r4 + 4 * h) = v;
+        }
+    __syncthreads();
+    const int64_t rows = (int64_t)A.B * A.Hkv * RT, at0 = (int64_t)bh * RT;
+    for (int u = tid; u < RT * (DP / 4); u += 64 * NW) {
+        const int r = u / (DP / 4), d = u % (DP / 4) * 4;
+        if (d >= A.D) continue;
+        f32x4 a = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(buf[0]) + r * DP + d);
+#pragma unroll
+        for (int k = 1; k < NW; ++k) a += *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(buf[k]) + r * DP + d);
+        const float v[4] = {a[0], a[1], a[2], a[3]};
+        if (A.nsplit > 1) {
+            store_f32<float, 4>(A.part_o + ((int64_t)split * rows + at0 + r) * A.D + d, v);
+        } else {
+            const int i = div_g(r, A.g_magic), g = r - i * A.G;
+            store_out<T>(A, (((int64_t)b * A.Sq + i) * A.Hq + hk * A.G + g) * A.D + d, v);
+        }
+    }
+    if (tid < RT) {                                             // tid < 32: lane = row
+        if (A.nsplit > 1) A.part_lse[(int64_t)split * rows + at0 + R] = sum == 0.f ? -INFINITY : mx + __builtin_amdgcn_logf(sum);
+        else if (A.lse) A.lse[at0 + R] = sum == 0.f ? INFINITY : mx + __builtin_amdgcn_logf(sum);
+    }
 }
 
 // joins the parts of a row: weights 2^(lse_s - max), added in order of the parts.  One thread per 4 features.
@@ -254,25 +385,28 @@ __global__ __launch_bounds__(NT) void attn_join_kernel(AttnK A) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) a[e] *= inv;
     const int64_t bh = at / RT;
-    const int R = (int)(at - bh * RT), i = R / A.G, g = R - i * A.G, hk = (int)(bh % A.Hkv);
-    store_f32<T, 4>((T *)A.o + (((bh / A.Hkv) * A.Sq + i) * A.Hq + hk * A.G + g) * A.D + d, a);
+    const int R = (int)(at - bh * RT), i = div_g(R, A.g_magic), g = R - i * A.G, hk = (int)(bh % A.Hkv);
+    store_out<T>(A, (((bh / A.Hkv) * A.Sq + i) * A.Hq + hk * A.G + g) * A.D + d, a);
     if (A.lse && d == 0) A.lse[at] = sum == 0.f ? INFINITY : mx + __builtin_amdgcn_logf(sum);
 }
 
 template <typename T> constexpr int key_tile() { return sizeof(T) == 4 ? 32 : 64; }
 int pad_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-struct Split { int nsplit, ndoc_tiles; int64_t part_floats, lse_floats, rng_floats; };
+struct Split { bool token; int nsplit, ndoc_tiles; int64_t part_floats, lse_floats, rng_floats; };
 Split plan(const sqd_attn_args *a) {
-    const int KT = a->dtype == SQD_F32 ? 32 : 64, G = a->Hq / a->Hkv;
-    const int64_t rows = (int64_t)a->Sq * G, groups = (int64_t)a->B * a->Hkv * ((rows + BM - 1) / BM);
+    const int G = a->Hq / a->Hkv;
+    const int64_t rows = (int64_t)a->Sq * G;
     Split p{};
-    // two workgroups fit a CU: split the keys while fewer than 512 would run, down to 4 key tiles (256 keys) for each
+    p.token = rows <= 32;
+    const int KT = p.token ? 32 : a->dtype == SQD_F32 ? 32 : 64;
+    const int64_t groups = (int64_t)a->B * a->Hkv * (p.token ? 1 : (rows + BM - 1) / BM);
+    // two workgroups fit a CU: split the keys while fewer than 512 would run, down to 256 keys for each
     const int tiles = (a->Sk + KT - 1) / KT;
     int64_t n = groups ? 512 / groups : 1;
-    n = n > tiles / 4 ? tiles / 4 : n;
+    n = n > a->Sk / 256 ? a->Sk / 256 : n;
     p.nsplit = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-    p.ndoc_tiles = a->q_docs ? tiles : 0;
+    p.ndoc_tiles = a->q_docs && !p.token ? tiles : 0;
     p.part_floats = p.nsplit > 1 ? (int64_t)p.nsplit * a->B * a->Hkv * rows * a->D : 0;
     p.lse_floats = p.nsplit > 1 ? ((int64_t)p.nsplit * a->B * a->Hkv * rows + 3) / 4 * 4 : 0;
     p.rng_floats = (int64_t)2 * a->B * p.ndoc_tiles;
@@ -286,7 +420,8 @@ int attn_check(const char *who, const sqd_attn_args *a) {
     SQD_CHECK_ARG(a->B >= 0 && a->Sq >= 0 && a->Sk >= 0 && a->Hq > 0 && a->Hkv > 0 && a->Hq % a->Hkv == 0, "%s: bad shape B=%d Sq=%d Sk=%d Hq=%d Hkv=%d",
                   who, a->B, a->Sq, a->Sk, a->Hq, a->Hkv);
     SQD_CHECK_ARG(a->D >= 8 && a->D <= 128 && a->D % 8 == 0, "%s: %d features a head (a multiple of 8 up to 128)", who, a->D);
-    SQD_CHECK_ARG(a->Sk < (1 << 24) && (int64_t)a->Sq * (a->Hq / a->Hkv) < (1 << 30) && (int64_t)a->B * a->Hkv < (1 << 24), "%s: too many tokens", who);
+    SQD_CHECK_ARG(a->Sk < (1 << 24) && (int64_t)a->Sq * (a->Hq / a->Hkv) < (1 << 30) &&
+                      (int64_t)a->Sq * (a->Hq / a->Hkv) * (a->Hq / a->Hkv) < (1ll << 31) && (int64_t)a->B * a->Hkv < (1 << 24), "%s: too many tokens", who);
     SQD_CHECK_ARG(a->scale > 0.f && a->scale < 3e38f && a->softcap >= 0.f && a->softcap < 3e38f, "%s: scale %g, cap %g", who, (double)a->scale, (double)a->softcap);
     SQD_CHECK_ARG(a->dtype >= SQD_F32 && a->dtype <= SQD_F16, "%s: element type %d", who, a->dtype);
     SQD_CHECK_ARG(!a->prefix || a->causal, "%s: a prefix needs the causal order", who);
@@ -300,7 +435,7 @@ int attn_check_tensor(const char *who, const char *name, const void *p, const in
 }
 AttnK attn_kargs(const sqd_attn_args *a) {
     AttnK A{};
-    A.q = a->q, A.k = a->k, A.v = a->v, A.go = a->go, A.o = a->o, A.gq = a->gq, A.gk = a->gk, A.gv = a->gv, A.lse = a->lse;
+    A.q = a->q, A.k = a->k, A.v = a->v, A.go = a->go, A.o = a->o, A.o_low = a->o_low, A.gq = a->gq, A.gk = a->gk, A.gv = a->gv, A.lse = a->lse;
     A.slopes = a->slopes, A.prefix = a->prefix, A.q_docs = a->q_docs, A.k_docs = a->k_docs, A.k_len = a->k_len;
     for (int i = 0; i < 3; ++i) A.qs[i] = a->q_stride[i], A.ks[i] = a->k_stride[i], A.vs[i] = a->v_stride[i], A.gos[i] = a->go_stride[i];
     constexpr double LOG2E = 1.44269504088896340736;
@@ -308,6 +443,7 @@ AttnK attn_kargs(const sqd_attn_args *a) {
     A.scale_log2 = (float)(a->scale * LOG2E);
     if (a->softcap > 0.f) A.cap_in = (float)(2.0 * LOG2E * a->scale / a->softcap), A.cap_out = (float)(a->softcap * LOG2E);
     A.B = a->B, A.Sq = a->Sq, A.Sk = a->Sk, A.Hq = a->Hq, A.Hkv = a->Hkv, A.G = a->Hq / a->Hkv, A.D = a->D, A.causal = a->causal;
+    A.g_magic = A.G == 1 ? 0u : (unsigned)(((1ull << 32) + A.G - 1) / A.G);
     return A;
 }
 void attn_doc_ranges(const int *ids, int2 *out, int B, int S, int div, int span, int ntile, hipStream_t st) {
@@ -344,9 +480,13 @@ extern "C" int sqd_attn_fwd(const sqd_attn_args *a) {
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);
         constexpr int KT = key_tile<T>();
-        if (a->q_docs && p.ndoc_tiles) attn_doc_ranges(A.k_docs, rng, A.B, A.Sk, 1, KT, p.ndoc_tiles, st);
+        if (p.ndoc_tiles) attn_doc_ranges(A.k_docs, rng, A.B, A.Sk, 1, KT, p.ndoc_tiles, st);
         auto go = [&](auto dp, auto cap, auto bias) {
-            hipLaunchKernelGGL((attn_fwd_kernel<T, decltype(dp)::value, KT, decltype(cap)::value, decltype(bias)::value>), dim3((unsigned)blocks), dim3(NT),
+            if (p.token)
+                hipLaunchKernelGGL((attn_token_kernel<T, decltype(dp)::value, token_waves<T, decltype(dp)::value>(), decltype(cap)::value, decltype(bias)::value>),
+                                   dim3((unsigned)blocks), dim3(64 * token_waves<T, decltype(dp)::value>()), 0, st, A);
+            else
+                hipLaunchKernelGGL((attn_fwd_kernel<T, decltype(dp)::value, KT, decltype(cap)::value, decltype(bias)::value>), dim3((unsigned)blocks), dim3(NT),
                                0, st, A);
         };
         auto flags = [&](auto dp) {

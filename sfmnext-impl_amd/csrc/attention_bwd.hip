@@ -25,19 +25,26 @@ using namespace sqd;
 constexpr int NT = 256, BM = 128;
 constexpr float ONE_LESS = 1.f - 2.384185791015625e-7f;        // 1 - 2^-22
 
-// delta [B,Hkv,Sq*G] (packed rows): 16 lanes a row, 8 features a lane
+// delta [B,Hkv,Sq*G] (packed rows): 16 lanes a row, 8 features a lane.  o's rounding alone would be as large an error of a gradient as the rounding
+// of dS, so what it left (o_low) is added back.
 template <typename T>
 __global__ __launch_bounds__(NT) void attn_delta_kernel(AttnK A) {
     const int RT = A.Sq * A.G, c = (threadIdx.x & 15) * 8;
     const int64_t at = (int64_t)blockIdx.x * (NT / 16) + (threadIdx.x >> 4), rows = (int64_t)A.B * A.Hkv * RT;
     if (at >= rows) return;
     const int64_t bh = at / RT;
-    const int R = (int)(at - bh * RT), i = R / A.G, hq = (int)(bh % A.Hkv) * A.G + R - i * A.G;
+    const int R = (int)(at - bh * RT), i = div_g(R, A.g_magic), hq = (int)(bh % A.Hkv) * A.G + R - i * A.G;
     const int64_t b = bh / A.Hkv;
     float s = 0.f;
     if (c < A.D) {
+        const int64_t o = ((b * A.Sq + i) * A.Hq + hq) * A.D + c;
         float u[8], v[8];
-        load_f32<T, 8>((const T *)A.o + ((b * A.Sq + i) * A.Hq + hq) * A.D + c, u);
+        load_f32<T, 8>((const T *)A.o + o, u);
+        if (sizeof(T) == 2 && A.o_low) {
+            load_f32<T, 8>((const T *)A.o_low + o, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] += v[e];
+        }
         load_f32<T, 8>((const T *)A.go + b * A.gos[0] + i * A.gos[1] + hq * A.gos[2] + c, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s = fmaf(u[e], v[e], s);
@@ -47,67 +54,72 @@ __global__ __launch_bounds__(NT) void attn_delta_kernel(AttnK A) {
     if ((threadIdx.x & 15) == 0) A.delta[at] = s;
 }
 
-// one score's probability and the factor 1 - tanh^2
-template <bool CAP, bool BIAS> __device__ __forceinline__ float score(float raw, const AttnK &A, float slope, float dist, float &fac) {
-    float x;
-    fac = 1.f;
+// probability and score gradient (without the scale) of one pair; `see` false: zeros, whatever the products hold
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ void pair_grad(float raw, float dp, float lse, float delta, float slope, float dist, const AttnK &A, bool see, float &p, float &ds) {
+    float x = raw, fac = 1.f;
     if (CAP) {
         const float t = tanh_of<CAP>(raw, A.cap_in);
         fac = fmaf(-t, t, 1.f);
         x = A.cap_out * t;
-    } else {
-        x = raw;                                               // the scale goes into the exponent's fma
     }
     if (BIAS) x = fmaf(-slope, fabsf(dist), CAP ? x : x * A.scale_log2);
-    return x;
+    p = exp2_hw(fmaf(x, CAP || BIAS ? 1.f : A.scale_log2, -lse));
+    p = see ? p : 0.f;
+    const float q = see && p < ONE_LESS ? p : 0.f, e = see ? dp - delta : 0.f;
+    ds = CAP ? q * e * fac : q * e;
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NT, 1) void attn_dkv_kernel(AttnK A) {
-    constexpr int QT = 32, DB = DP / 32;
+// 4 waves: KW of them side by side on 32 keys each, 4 / KW on the halves of a row tile.
+template <typename T, int DP, int KW, bool CAP, bool BIAS>
+__global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_kernel(AttnK A) {
+    constexpr int QW = 4 / KW, QT = 32 * QW, DB = DP / 32;
     typedef Tile<T, DP> L;
     typedef typename L::frag frag;
-    __shared__ __align__(16) char lq[2][QT * L::PITCH], lg[2][QT * L::PITCH];
+    typedef Stage<T, DP, QT, NT> S;
+    __shared__ __align__(16) char lq[2][S::BYTES], lg[2][S::BYTES];
     __shared__ __align__(16) float r_lse[2][QT], r_delta[2][QT], r_slope[2][QT];
     __shared__ __align__(16) int r_lim[2][QT], r_doc[2][QT], r_pos[2][QT];
+    __shared__ int wk[8];
+    static_assert(QW == 1 || sizeof(lq) >= (size_t)KW * (QW - 1) * 64 * DB * 16 * 4, "a wave's sums fit the row buffers");
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, kw = wave % KW, qw = wave / KW;
     int w = xcd_order(blockIdx.x, gridDim.x);
     const int tile = w % A.ntile, bh = w / A.ntile, hk = bh % A.Hkv, b = bh / A.Hkv;
-    const int RT = A.Sq * A.G, j0 = tile * 128, jl = j0 + wave * 32 + (lane & 31);
+    const int RT = A.Sq * A.G, j0 = tile * 32 * KW, jl = j0 + kw * 32 + (lane & 31);
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk, off = len - A.Sq;
     const int prefix = A.prefix ? A.prefix[b] : 0;
-    const bool docs = A.k_docs != nullptr;
-    int kd = -1;
+    const int *qdoc = A.q_docs ? A.q_docs + (int64_t)b * A.Sq : nullptr;
+    const bool docs = qdoc != nullptr;
+    int kd = -3;
     if (docs && jl < len) kd = A.k_docs[(int64_t)b * A.Sk + jl];
     const bool on = jl < len && (!docs || kd >= 0);
     if (docs && !on) kd = -3;
+    clear_lds<NT>(lq[0], 2 * S::BYTES, tid);
+    clear_lds<NT>(lg[0], 2 * S::BYTES, tid);
 
-    int dlo = 0, dhi = 0;
-    if (docs) {                                                // documents of the 128 keys: the four ranges of 32
-        __shared__ int wk[8];
-        int lo = kd >= 0 ? kd : 0x7fffffff, hi = kd;
+    int dlo = 0, dhi = 0, wlo = 0, whi = 0;                    // documents of the workgroup's keys, of the wave's
+    if (docs) {
+        wlo = kd >= 0 ? kd : 0x7fffffff, whi = kd;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
-            lo = min(lo, __shfl_xor(lo, o, 64));
-            hi = max(hi, __shfl_xor(hi, o, 64));
+            wlo = min(wlo, __shfl_xor(wlo, o, 64));
+            whi = max(whi, __shfl_xor(whi, o, 64));
         }
-        if (lane == 0) wk[wave] = lo, wk[4 + wave] = hi;
-        __syncthreads();
-        dlo = min(min(wk[0], wk[1]), min(wk[2], wk[3]));
-        dhi = max(max(wk[4], wk[5]), max(wk[6], wk[7]));
+        if (lane == 0) wk[wave] = wlo, wk[4 + wave] = whi;
     }
-    const int2 *rng = A.doc_rng + (int64_t)b * A.ndoc_tiles;
+    __syncthreads();
+    if (docs) {
+        dlo = __builtin_amdgcn_readfirstlane(min(min(wk[0], wk[1]), min(wk[2], wk[3])));
+        dhi = __builtin_amdgcn_readfirstlane(max(max(wk[4], wk[5]), max(wk[6], wk[7])));
+    }
     const int nt = (RT + QT - 1) / QT;
     // rows that see a key >= j0: all of them, in causal order those from query j0 - off on (a prefix past j0: all)
     int t0 = 0;
     if (A.causal && prefix <= j0) t0 = (int)(min((int64_t)max(j0 - off, 0) * A.G, (int64_t)RT) / QT);
     if (j0 >= len) t0 = nt;
-    auto next = [&](int t) {
-        if (docs)
-            while (t < nt && (rng[t].y < dlo || rng[t].x > dhi)) ++t;
-        return t;
-    };
+    DocWalk walk(docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, nt);
+    const bool all_on = __all(on);
 
     frag kf[L::KS], vf[L::KS];
     const T *krow = (const T *)A.k + b * A.ks[0] + (int64_t)jl * A.ks[1] + hk * A.ks[2];
@@ -119,99 +131,141 @@ __global__ __launch_bounds__(NT, 1) void attn_dkv_kernel(AttnK A) {
     }
 
     const T *qb = (const T *)A.q + b * A.qs[0] + (int64_t)hk * A.G * A.qs[2], *gb = (const T *)A.go + b * A.gos[0] + (int64_t)hk * A.G * A.gos[2];
-    Stage<T, DP, QT, NT> sq, sg;
+    S st(tid);
+    const unsigned oq[2] = {lds_offset(lq[0]), lds_offset(lq[1])}, og[2] = {lds_offset(lg[0]), lds_offset(lg[1])};
     float s_lse = 0.f, s_delta = 0.f, s_slope = 0.f;
-    int s_lim = -1, s_doc = -2, s_pos = 0;
-    auto fetch = [&](int t) {
-        auto row_of = [&](const T *base, const int64_t *st) {
-            const int64_t s1 = st[1], s2 = st[2];
-            return [=, &A](int r) -> const T * {
-                const int R = t * QT + r;
-                if (R >= RT) return nullptr;
-                const int i = R / A.G, g = R - i * A.G;
-                if (docs && A.q_docs[(int64_t)b * A.Sq + i] < 0) return nullptr;        // rows that see no key hold anything
-                if (row_limit(i + off, len, A.causal, prefix) < 0) return nullptr;
-                return base + i * s1 + g * s2;
+    int s_lim = -1, s_doc = -2, s_pos = 0, s_i = 0;
+    // rows that see no key hold anything and are not loaded: documents are read a tile ahead of the DMA that goes by them
+    int pd[S::N];
+    auto peek = [&](int t) {
+        if (!docs) return;
+#pragma unroll
+        for (int n = 0; n < S::N; ++n) {
+            const int R = t * QT + st.row[n];
+            pd[n] = t < nt && st.row[n] >= 0 && R < RT ? qdoc[div_g(R, A.g_magic)] : -1;
+        }
+        const int R = t * QT + tid;
+        s_doc = t < nt && tid < QT && R < RT ? qdoc[div_g(R, A.g_magic)] : -2;
+    };
+    auto fetch = [&](int t, int s) {
+        auto rows = [&](const T *base, int64_t s1, int64_t s2) {
+            return [=, &A, &pd](int n, int r) -> const T * {
+                const int R = t * QT + r, i = div_g(R, A.g_magic);
+                if (R >= RT || (docs && pd[n] < 0) || row_limit(i + off, len, A.causal, prefix) < 0) return nullptr;
+                return base + i * s1 + (R - i * A.G) * s2;
             };
         };
-        sq.load(tid, A.D, row_of(qb, A.qs));
-        sg.load(tid, A.D, row_of(gb, A.gos));
         if (tid < QT) {
             const int R = t * QT + tid;
-            s_lim = -1, s_doc = -2, s_lse = INFINITY, s_delta = 0.f;
+            s_lim = -1, s_lse = INFINITY, s_delta = 0.f;
             if (R < RT) {
-                const int i = R / A.G;
-                s_pos = i + off;
+                s_i = div_g(R, A.g_magic);
+                s_pos = s_i + off;
                 s_lse = A.lse[(int64_t)bh * RT + R];
                 s_delta = A.delta[(int64_t)bh * RT + R];
-                if (BIAS) s_slope = A.slopes[hk * A.G + R - i * A.G] * 1.44269504088896341f;
-                if (docs) s_doc = A.q_docs[(int64_t)b * A.Sq + i];
+                if (BIAS) s_slope = A.slopes[hk * A.G + R - s_i * A.G] * 1.44269504088896341f;
                 if (!docs || s_doc >= 0) s_lim = row_limit(s_pos, len, A.causal, prefix);
             }
+            if (docs) r_doc[s][tid] = s_doc;
         }
+        st.load(oq[s], tid, A.D, rows(qb, A.qs[1], A.qs[2]));
+        st.load(og[s], tid, A.D, rows(gb, A.gos[1], A.gos[2]));
     };
     auto put = [&](int s) {
-        sq.store(lq[s], tid);
-        sg.store(lg[s], tid);
         if (tid < QT) {
-            r_lse[s][tid] = s_lse, r_delta[s][tid] = s_delta, r_lim[s][tid] = s_lim, r_doc[s][tid] = s_doc, r_pos[s][tid] = s_pos;
-            if (BIAS) r_slope[s][tid] = s_slope;
+            r_lse[s][tid] = s_lse, r_delta[s][tid] = s_delta, r_lim[s][tid] = s_lim;
+            if (BIAS) r_slope[s][tid] = s_slope, r_pos[s][tid] = s_pos;
         }
     };
 
     f32x16 gk[DB], gv[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) gk[db] = f32x16{}, gv[db] = f32x16{};
-    int t = next(t0), s = 0;
+    int s = 0;
+    bool u, un;
+    int t = walk.next(t0, u);
+    peek(t);
     if (t < nt) {
-        fetch(t);
+        fetch(t, 0);
         put(0);
     }
+    int tn = walk.next(t + 1, un);
+    peek(tn);
+    dma_wait();
     __syncthreads();
     while (t < nt) {
-        const int tn = next(t + 1);
-        if (tn < nt) fetch(tn);
+        if (tn < nt) fetch(tn, s ^ 1);
+        bool u2 = true;
+        const int t2 = walk.next(tn + 1, u2);
+        peek(t2);
+        const int q0 = qw * 32;
         f32x16 x = {}, dp = {};
 #pragma unroll
         for (int ks = 0; ks < L::KS; ++ks) {
-            x = Mma<T>::mma(L::row_frag(lq[s], lane & 31, ks, h), kf[ks], x);
-            dp = Mma<T>::mma(L::row_frag(lg[s], lane & 31, ks, h), vf[ks], dp);
+            x = Mma<T>::mma(L::row_frag(lq[s], q0 + (lane & 31), ks, h), kf[ks], x);
+            dp = Mma<T>::mma(L::row_frag(lg[s], q0 + (lane & 31), ks, h), vf[ks], dp);
         }
+        // every row of the tile sees all of the wave's keys?  (limits do not fall with the row)
+        const int R0 = t * QT + q0;
+        const bool part = !all_on || !u || R0 + 32 > RT || row_limit(div_g(R0, A.g_magic) + off, len, A.causal, prefix) < j0 + kw * 32 + 31;
         float p[16], ds[16];
+        auto grads = [&](auto masked) {
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            const int q4 = 8 * r4 + 4 * h;
-            const f32x4 lse = *reinterpret_cast<const f32x4 *>(&r_lse[s][q4]), delta = *reinterpret_cast<const f32x4 *>(&r_delta[s][q4]);
-            const int4 lim = *reinterpret_cast<const int4 *>(&r_lim[s][q4]);
-            int4 qd = make_int4(kd, kd, kd, kd), ps = make_int4(0, 0, 0, 0);
-            f32x4 sl = {0, 0, 0, 0};
-            if (docs) qd = *reinterpret_cast<const int4 *>(&r_doc[s][q4]);
-            if (BIAS) ps = *reinterpret_cast<const int4 *>(&r_pos[s][q4]), sl = *reinterpret_cast<const f32x4 *>(&r_slope[s][q4]);
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int q4 = q0 + 8 * r4 + 4 * h;
+                const f32x4 lse = *reinterpret_cast<const f32x4 *>(&r_lse[s][q4]), delta = *reinterpret_cast<const f32x4 *>(&r_delta[s][q4]);
+                int4 lim = make_int4(0, 0, 0, 0), qd = make_int4(kd, kd, kd, kd), ps = make_int4(0, 0, 0, 0);
+                f32x4 sl = {0, 0, 0, 0};
+                if (masked) lim = *reinterpret_cast<const int4 *>(&r_lim[s][q4]);
+                if (masked && docs) qd = *reinterpret_cast<const int4 *>(&r_doc[s][q4]);
+                if (BIAS) ps = *reinterpret_cast<const int4 *>(&r_pos[s][q4]), sl = *reinterpret_cast<const f32x4 *>(&r_slope[s][q4]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = r4 * 4 + e;
-                const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
-                const int pe = e == 0 ? ps.x : e == 1 ? ps.y : e == 2 ? ps.z : ps.w;
-                float fac;
-                const float v = score<CAP, BIAS>(x[r], A, sl[e], (float)(pe - jl), fac);
-                const bool see = jl <= le && de == kd;
-                p[r] = see ? exp2_hw(fmaf(v, CAP || BIAS ? 1.f : A.scale_log2, -lse[e])) : 0.f;
-                ds[r] = p[r] > 0.f && p[r] < ONE_LESS ? p[r] * (dp[r] - delta[e]) * fac : 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    const int r = r4 * 4 + e;
+                    const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
+                    const int pe = e == 0 ? ps.x : e == 1 ? ps.y : e == 2 ? ps.z : ps.w;
+                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], delta[e], sl[e], (float)(pe - jl), A, !masked || (jl <= le && de == kd), p[r], ds[r]);
+                }
             }
-        }
+        };
+        if (part) grads(std::true_type{});
+        else grads(std::false_type{});
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             const frag pf = Mma<T>::pack(&p[8 * kk]), df = Mma<T>::pack(&ds[8 * kk]);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                gv[db] = Mma<T>::mma(L::col_frag(lg[s], kk * 16, db, lane), pf, gv[db]);
-                gk[db] = Mma<T>::mma(L::col_frag(lq[s], kk * 16, db, lane), df, gk[db]);
+                gv[db] = Mma<T>::mma(L::col_frag(lg[s], q0 + kk * 16, db, lane), pf, gv[db]);
+                gk[db] = Mma<T>::mma(L::col_frag(lq[s], q0 + kk * 16, db, lane), df, gk[db]);
             }
         }
         if (tn < nt) put(s ^ 1);
+        dma_wait();
         __syncthreads();
         s ^= 1;
-        t = tn;
+        t = tn, u = un, tn = t2, un = u2;
+    }
+    if (QW > 1) {                                              // the row halves' sums, through the row buffers: gK, then gV
+        float *red = reinterpret_cast<float *>(lq[0]);
+        auto join = [&](f32x16 (&g)[DB]) {
+            if (qw > 0)
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) red[(((qw - 1) * KW + kw) * DB * 16 + db * 16 + r) * 64 + lane] = g[db][r];
+            __syncthreads();
+            if (qw == 0)
+#pragma unroll
+                for (int k = 0; k < QW - 1; ++k)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) g[db][r] += red[((k * KW + kw) * DB * 16 + db * 16 + r) * 64 + lane];
+            __syncthreads();
+        };
+        join(gk);
+        join(gv);
+        if (qw > 0) return;
     }
     if (jl >= A.Sk) return;
     const int64_t o = (((int64_t)b * A.Sk + jl) * A.Hkv + hk) * A.D;
@@ -233,7 +287,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     constexpr int KT = 32, DB = DP / 32;
     typedef Tile<T, DP> L;
     typedef typename L::frag frag;
-    __shared__ __align__(16) char lk[2][KT * L::PITCH], lv[2][KT * L::PITCH];
+    typedef Stage<T, DP, KT, NT> S;
+    __shared__ __align__(16) char lk[2][S::BYTES], lv[2][S::BYTES];
     __shared__ __align__(16) int ld[2][KT];
     __shared__ int wq[8];
 
@@ -241,87 +296,84 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     int w = xcd_order(blockIdx.x, gridDim.x);
     const int tile = A.ntile - 1 - w % A.ntile, bh = w / A.ntile, hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, row0 = tile * BM;
-    const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk, off = len - A.Sq;
+    const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
     const int prefix = A.prefix ? A.prefix[b] : 0;
     const int R = row0 + wave * 32 + (lane & 31);
-    const bool in = R < RT;
-    const int i = in ? R / A.G : A.Sq - 1, g = in ? R - i * A.G : 0, pos = i + off;
-    int qd = -2;
-    if (A.q_docs && in) qd = max(A.q_docs[(int64_t)b * A.Sq + i], -2);
-    if (qd < 0) qd = -2;
-    const bool on = in && (!A.q_docs || qd >= 0);
-    const int lim = on ? row_limit(pos, len, A.causal, prefix) : -1;
+    const RowOf row = row_of(A, b, R, RT, len, prefix);
+    clear_lds<NT>(lk[0], 2 * S::BYTES, tid);
+    clear_lds<NT>(lv[0], 2 * S::BYTES, tid);
     int kend = len;
-    if (A.causal) kend = max(0, min(len, max(min(A.Sq - 1, (row0 + BM - 1) / A.G) + off + 1, prefix)));
+    if (A.causal) kend = max(0, min(len, max(min(A.Sq - 1, div_g(row0 + BM - 1, A.g_magic)) + len - A.Sq + 1, prefix)));
     int dlo = 0, dhi = 0;
     if (A.q_docs) {
-        int lo = qd >= 0 ? qd : 0x7fffffff, hi = qd;
+        int lo = row.qd >= 0 ? row.qd : 0x7fffffff, hi = row.qd;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
             lo = min(lo, __shfl_xor(lo, o, 64));
             hi = max(hi, __shfl_xor(hi, o, 64));
         }
         if (lane == 0) wq[wave] = lo, wq[4 + wave] = hi;
-        __syncthreads();
-        dlo = min(min(wq[0], wq[1]), min(wq[2], wq[3]));
-        dhi = max(max(wq[4], wq[5]), max(wq[6], wq[7]));
+    }
+    __syncthreads();
+    if (A.q_docs) {
+        dlo = __builtin_amdgcn_readfirstlane(min(min(wq[0], wq[1]), min(wq[2], wq[3])));
+        dhi = __builtin_amdgcn_readfirstlane(max(max(wq[4], wq[5]), max(wq[6], wq[7])));
     }
     const int t1 = (kend + KT - 1) / KT;
-    // the ranges are those of 64 keys
-    const int2 *rng = A.doc_rng + (int64_t)b * A.ndoc_tiles;
-    auto next = [&](int t) {
-        if (A.q_docs)
-            while (t < t1 && (rng[t].y < dlo || rng[t].x > dhi)) ++t;
-        return t;
-    };
+    DocWalk walk(A.q_docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, t1);
 
     frag qf[L::KS], gf[L::KS];
-    const T *qrow = (const T *)A.q + b * A.qs[0] + (int64_t)i * A.qs[1] + (int64_t)(hk * A.G + g) * A.qs[2];
-    const T *grow = (const T *)A.go + b * A.gos[0] + (int64_t)i * A.gos[1] + (int64_t)(hk * A.G + g) * A.gos[2];
+    const bool live = row.lim >= 0;                            // rows that see no key hold anything
+    const T *qrow = (const T *)A.q + b * A.qs[0] + (int64_t)row.i * A.qs[1] + (int64_t)(hk * A.G + row.g) * A.qs[2];
+    const T *grow = (const T *)A.go + b * A.gos[0] + (int64_t)row.i * A.gos[1] + (int64_t)(hk * A.G + row.g) * A.gos[2];
 #pragma unroll
     for (int ks = 0; ks < L::KS; ++ks) {
-        qf[ks] = L::mem_frag(qrow, ks, h, A.D, on);
-        gf[ks] = L::mem_frag(grow, ks, h, A.D, on);
+        qf[ks] = L::mem_frag(qrow, ks, h, A.D, live);
+        gf[ks] = L::mem_frag(grow, ks, h, A.D, live);
     }
     float lse = INFINITY, delta = 0.f;
-    if (on) lse = A.lse[(int64_t)bh * RT + R], delta = A.delta[(int64_t)bh * RT + R];
+    if (live) lse = A.lse[(int64_t)bh * RT + R], delta = A.delta[(int64_t)bh * RT + R];
 
     const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
     const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
-    Stage<T, DP, KT, NT> sk, sv;
-    int sd = -1;
-    auto fetch = [&](int t) {
-        const int j0 = t * KT;
-        auto row_of = [&](const T *base, int64_t stride) {
-            return [=](int r) -> const T * {
-                const int j = j0 + r;
-                if (j >= len || (kdoc && kdoc[j] < 0)) return nullptr;
-                return base + j * stride;
-            };
-        };
-        sk.load(tid, A.D, row_of(kbase, A.ks[1]));
-        sv.load(tid, A.D, row_of(vbase, A.vs[1]));
-        if (kdoc && tid < KT) sd = j0 + tid < len ? kdoc[j0 + tid] : -1;
+    S st(tid);
+    const unsigned ok[2] = {lds_offset(lk[0]), lds_offset(lk[1])}, ov[2] = {lds_offset(lv[0]), lds_offset(lv[1])};
+    int pd[S::N], sd = -1;                                     // as in the forward
+    auto peek = [&](int t) {
+        if (!kdoc) return;
+#pragma unroll
+        for (int n = 0; n < S::N; ++n) pd[n] = t < t1 && st.row[n] >= 0 && t * KT + st.row[n] < len ? kdoc[t * KT + st.row[n]] : -1;
+        sd = t < t1 && tid < KT && t * KT + tid < len ? kdoc[t * KT + tid] : -1;
     };
-    auto put = [&](int s) {
-        sk.store(lk[s], tid);
-        sv.store(lv[s], tid);
+    auto fetch = [&](int t, int s) {
+        const int j0 = t * KT;
+        auto rows = [&](const T *base, int64_t stride) {
+            const T *p0 = base + j0 * stride;
+            return [=, &pd](int n, int r) -> const T * { return j0 + r < len && (!kdoc || pd[n] >= 0) ? p0 + r * stride : nullptr; };
+        };
+        st.load(ok[s], tid, A.D, rows(kbase, A.ks[1]));
+        st.load(ov[s], tid, A.D, rows(vbase, A.vs[1]));
         if (kdoc && tid < KT) ld[s][tid] = sd;
     };
-    const float slope = BIAS && in ? A.slopes[hk * A.G + g] * 1.44269504088896341f : 0.f;
+    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * 1.44269504088896341f : 0.f;
     f32x16 gq[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) gq[db] = f32x16{};
 
-    int t = next(0), s = 0;
-    if (t < t1) {
-        fetch(t);
-        put(0);
-    }
+    int s = 0;
+    bool u, un;
+    int t = walk.next(0, u);
+    peek(t);
+    if (t < t1) fetch(t, 0);
+    int tn = walk.next(t + 1, un);
+    peek(tn);
+    dma_wait();
     __syncthreads();
     while (t < t1) {
-        const int tn = next(t + 1);
-        if (tn < t1) fetch(tn);
+        if (tn < t1) fetch(tn, s ^ 1);
+        bool u2 = true;
+        const int t2 = walk.next(tn + 1, u2);
+        peek(t2);
         const int j0 = t * KT;
         f32x16 x = {}, dp = {};
 #pragma unroll
@@ -329,34 +381,37 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
             x = Mma<T>::mma(L::row_frag(lk[s], lane & 31, ks, h), qf[ks], x);
             dp = Mma<T>::mma(L::row_frag(lv[s], lane & 31, ks, h), gf[ks], dp);
         }
+        const bool part = !u || __any(row.lim < j0 + KT - 1);
         float ds[16];
+        auto grads = [&](auto masked) {
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            const int j4 = 8 * r4 + 4 * h;
-            int4 kd = make_int4(qd, qd, qd, qd);
-            if (kdoc) kd = *reinterpret_cast<const int4 *>(&ld[s][j4]);
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int j4 = 8 * r4 + 4 * h;
+                int4 kd = make_int4(row.qd, row.qd, row.qd, row.qd);
+                if (masked && kdoc) kd = *reinterpret_cast<const int4 *>(&ld[s][j4]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
-                float fac;
-                const float v = score<CAP, BIAS>(x[r], A, slope, (float)(pos - j), fac);
-                const float p = j <= lim && d == qd ? exp2_hw(fmaf(v, CAP || BIAS ? 1.f : A.scale_log2, -lse)) : 0.f;
-                ds[r] = p > 0.f && p < ONE_LESS ? p * (dp[r] - delta) * fac : 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
+                    float p;
+                    pair_grad<CAP, BIAS>(x[r], dp[r], lse, delta, slope, (float)(row.pos - j), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
+                }
             }
-        }
+        };
+        if (part) grads(std::true_type{});
+        else grads(std::false_type{});
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             const frag df = Mma<T>::pack(&ds[8 * kk]);
 #pragma unroll
             for (int db = 0; db < DB; ++db) gq[db] = Mma<T>::mma(L::col_frag(lk[s], kk * 16, db, lane), df, gq[db]);
         }
-        if (tn < t1) put(s ^ 1);
+        dma_wait();
         __syncthreads();
         s ^= 1;
-        t = tn;
+        t = tn, u = un, tn = t2, un = u2;
     }
-    if (!in) return;
-    T *out = (T *)A.gq + (((int64_t)b * A.Sq + i) * A.Hq + hk * A.G + g) * A.D;
+    if (!row.on) return;
+    T *out = (T *)A.gq + (((int64_t)b * A.Sq + row.i) * A.Hq + hk * A.G + row.g) * A.D;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -367,12 +422,15 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         }
 }
 
-struct BwdPlan { int64_t rows; int nq_tiles, nk_tiles; int64_t delta, q_rng, k_rng; };
+struct BwdPlan { int64_t rows; int kw, nq_tiles, nk_tiles; int64_t delta, q_rng, k_rng; };
 BwdPlan bwd_plan(const sqd_attn_args *a) {
     BwdPlan p{};
     const int G = a->Hq / a->Hkv;
     p.rows = (int64_t)a->B * a->Hkv * a->Sq * G;
-    p.nq_tiles = a->q_docs ? (a->Sq * G + 31) / 32 : 0;
+    // keys a workgroup: 128, or 64 with the row tile split between the waves while 128 would leave CUs idle or a last round nearly empty
+    p.kw = (int64_t)((a->Sk + 127) / 128) * a->B * a->Hkv < 1024 ? 2 : 4;
+    const int QT = 32 * (4 / p.kw);
+    p.nq_tiles = a->q_docs ? (a->Sq * G + QT - 1) / QT : 0;
     p.nk_tiles = a->q_docs ? (a->Sk + 31) / 32 : 0;
     p.delta = (p.rows + 3) / 4 * 4;
     p.q_rng = (int64_t)2 * a->B * p.nq_tiles;
@@ -410,15 +468,17 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);
         if (p.rows) hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((p.rows + 15) / 16)), dim3(NT), 0, st, A);
-        if (p.nq_tiles) attn_doc_ranges(A.q_docs, q_rng, A.B, A.Sq, A.G, 32, p.nq_tiles, st);
+        if (p.nq_tiles) attn_doc_ranges(A.q_docs, q_rng, A.B, A.Sq, A.G, 32 * (4 / p.kw), p.nq_tiles, st);
         if (p.nk_tiles) attn_doc_ranges(A.k_docs, k_rng, A.B, A.Sk, 1, 32, p.nk_tiles, st);
         auto go = [&](auto dp, auto cap, auto bias) {
             constexpr int DP = decltype(dp)::value;
             constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
             if (A.Sk) {
                 AttnK K = A;
-                K.ntile = (A.Sk + 127) / 128, K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
-                hipLaunchKernelGGL((attn_dkv_kernel<T, DP, CAP, BIAS>), dim3((unsigned)((int64_t)K.ntile * A.B * A.Hkv)), dim3(NT), 0, st, K);
+                K.ntile = (A.Sk + 32 * p.kw - 1) / (32 * p.kw), K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
+                const dim3 grid((unsigned)((int64_t)K.ntile * A.B * A.Hkv));
+                if (p.kw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 2, CAP, BIAS>), grid, dim3(NT), 0, st, K);
+                else hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, CAP, BIAS>), grid, dim3(NT), 0, st, K);
             }
             if (A.Sq) {
                 AttnK Q = A;

@@ -141,7 +141,7 @@ class RotaryAxes(torch.autograd.Function):
 class AttnArgs(ctypes.Structure):
     """struct sqd_attn_args (include/sqd.h)."""
     _P, _L, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
-    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("go", _P), ("o", _P), ("gq", _P), ("gk", _P), ("gv", _P), ("lse", _P), ("scratch", _P),
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("go", _P), ("o", _P), ("o_low", _P), ("gq", _P), ("gk", _P), ("gv", _P), ("lse", _P), ("scratch", _P),
                 ("slopes", _P), ("prefix", _P), ("q_docs", _P), ("k_docs", _P), ("k_len", _P), ("stream", _P),
                 ("q_stride", _L * 3), ("k_stride", _L * 3), ("v_stride", _L * 3), ("go_stride", _L * 3), ("scale", _F), ("softcap", _F),
                 ("B", _I), ("Sq", _I), ("Sk", _I), ("Hq", _I), ("Hkv", _I), ("D", _I), ("causal", _I), ("dtype", _I)]
@@ -161,18 +161,19 @@ def _attn_args(q, k, v, cfg, masks):
 
 
 def attn_fwd(q, k, v, cfg, masks, want_lse):
-    """-> o [B,Sq,Hq,D], lse [B,Hkv,Sq*G] or None; cfg = (scale, softcap, causal), masks = (slopes, prefix, q_docs, k_docs, k_len)"""
+    """-> o [B,Sq,Hq,D]; for the backward (want_lse): what its rounding left (16-bit types) and lse [B,Hkv,Sq*G]; cfg = (scale, softcap, causal), masks = (slopes, prefix, q_docs, k_docs, k_len)"""
     L = _l.lib()
     a = _attn_args(q, k, v, cfg, masks)
     o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lse = torch.empty((q.shape[0], k.shape[2], q.shape[1] * (q.shape[2] // k.shape[2])), device=q.device, dtype=torch.float32) if want_lse else None
-    a.o, a.lse = o.data_ptr(), _ptr(lse)
+    low = torch.empty_like(o) if want_lse and o.dtype != torch.float32 else None
+    a.o, a.o_low, a.lse = o.data_ptr(), _ptr(low), _ptr(lse)
     n = L.sqd_attn_fwd_scratch(ctypes.byref(a))
     if n > 0:
         scratch = torch.empty(n, device=q.device, dtype=torch.float32)
         a.scratch = scratch.data_ptr()
     _l.check(L.sqd_attn_fwd(ctypes.byref(a)), "attn_fwd")
-    return o, lse
+    return o, low, lse
 
 
 class Attention(torch.autograd.Function):
@@ -182,15 +183,15 @@ class Attention(torch.autograd.Function):
     def forward(ctx, q, k, v, cfg, *masks):
         with on_device(q):
             q, k, v = _rows16(q), _rows16(k), _rows16(v)
-            o, lse = attn_fwd(q, k, v, cfg, masks, True)
-        ctx.save_for_backward(q, k, v, o, lse, *masks)
+            o, low, lse = attn_fwd(q, k, v, cfg, masks, True)
+        ctx.save_for_backward(q, k, v, o, low, lse, *masks)
         ctx.cfg = cfg
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        q, k, v, o, lse, *masks = ctx.saved_tensors
+        q, k, v, o, low, lse, *masks = ctx.saved_tensors
         L = _l.lib()
         with on_device(q):
             go = _rows16(go)
@@ -198,6 +199,7 @@ class Attention(torch.autograd.Function):
             gq, gk, gv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
             a.go, a.o, a.lse, a.gq, a.gk, a.gv = (t.data_ptr() for t in (go, o, lse, gq, gk, gv))
             a.go_stride[:] = _strides(go)
+            a.o_low = _ptr(low)
             scratch = torch.empty(max(4, L.sqd_attn_bwd_scratch(ctypes.byref(a))), device=q.device, dtype=torch.float32)
             a.scratch = scratch.data_ptr()
             _l.check(L.sqd_attn_bwd(ctypes.byref(a)), "attn_bwd")
