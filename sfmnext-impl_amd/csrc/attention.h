@@ -23,14 +23,16 @@ namespace sqd {
 struct AttnK {
     const void *q, *k, *v, *go;
     void *o, *o_low, *gq, *gk, *gv;
-    float *lse, *delta, *part_o, *part_lse;
+    float *lse, *part_o, *part_lse;
+    float *row_lse, *row_delta, *row_slope;  // the backward's copies by packed row, padded to whole tiles (rows_padded a key head)
+    int *row_lim, *row_doc, *row_pos;
     const float *slopes;
     const int *prefix, *q_docs, *k_docs, *k_len;
     const int2 *doc_rng;                    // per tile of the looped-over side: smallest and largest document id
     int64_t qs[3], ks[3], vs[3], gos[3];
     float scale_log2, cap_in, cap_out, scale;             // log2(e) scale; 2 log2(e) scale / cap, cap log2(e)
     unsigned g_magic;
-    int B, Sq, Sk, Hq, Hkv, G, D, causal, ntile, nsplit, ndoc_tiles;
+    int B, Sq, Sk, Hq, Hkv, G, D, causal, ntile, nsplit, ndoc_tiles, rows_padded;
 };
 
 template <typename T> struct Mma;
@@ -131,10 +133,10 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// 16 bytes of this lane's address to LDS byte `lds` + 16 * lane, without a register in between.  The compiler does not see the load: dma_wait()
-// (and a barrier, for other waves' data) comes before the LDS bytes are read.  Lanes switched off leave their 16 bytes as they are.
-__device__ __forceinline__ void dma16(const void *g, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+// 16 bytes at base + off (this lane's) to LDS byte `lds` + 16 * lane, without a register in between.  The compiler does not see the load:
+// dma_wait() (and a barrier, for other waves' data) comes before the LDS bytes are read.  Lanes switched off leave their 16 bytes as they are.
+__device__ __forceinline__ void dma16(const void *base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_offset(const void *p) {
@@ -142,28 +144,45 @@ __device__ __forceinline__ unsigned lds_offset(const void *p) {
 }
 
 // a ROWS x DP tile from memory to LDS by NTH threads.  The LDS side of a DMA is linear in the lane, so the permutation of the pieces is applied to
-// the address a lane reads.  Pieces that are not loaded (rows nobody may see, features past D) keep what the buffer held: zeros at the start
-// (clear()), later an older tile's rows, which are data of this call: finite wherever the inputs that count are.
+// the offset a lane reads.  Offsets within a tile are 32-bit and fixed (the host checks that a tile's rows span less than 2 GiB), the tile's
+// base is a scalar: a tile costs one instruction a piece.  Pieces that are not loaded (rows nobody may see, features past D) keep what the buffer
+// held: zeros at the start (clear_lds), later an older tile's rows, which are data of this call: finite wherever the inputs that count are.
 template <typename T, int DP, int ROWS, int NTH> struct Stage {
     typedef Tile<T, DP> L;
     static constexpr int TOTAL = ROWS * L::CH, N = (TOTAL + NTH - 1) / NTH, BYTES = ROWS * L::PITCH;
-    int row[N], col[N];                     // this thread's pieces: tile row, first feature
-    __device__ __forceinline__ Stage(int tid) {
+    static constexpr int NO_ROW = 1 << 30;
+    unsigned off[N];
+    static __device__ __forceinline__ int piece_row(int n, int tid, int D) {
+        const int idx = tid + n * NTH;
+        return idx < TOTAL && piece_col(n, tid) < D ? idx / L::CH : NO_ROW;
+    }
+    static __device__ __forceinline__ int piece_col(int n, int tid) {
+        const int idx = tid + n * NTH;
+        return ((idx % L::CH) ^ (bitrev4((idx / L::CH) & 15) & L::ROT)) * L::CHE;
+    }
+    // rows `stride` elements apart
+    __device__ __forceinline__ void aim(int tid, unsigned stride) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) off[n] = ((unsigned)((tid + n * NTH) / L::CH) * stride + piece_col(n, tid)) * (unsigned)sizeof(T);
+    }
+    // packed rows: row r of the tile is query (rem + r) / G, head (rem + r) % G; queries s1, heads s2 elements apart
+    __device__ __forceinline__ void aim_packed(int tid, int rem, int G, unsigned magic, unsigned s1, unsigned s2) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int idx = tid + n * NTH;
-            row[n] = idx < TOTAL ? idx / L::CH : -1;
-            col[n] = ((idx % L::CH) ^ (bitrev4((idx / L::CH) & 15) & L::ROT)) * L::CHE;
+            const unsigned r = rem + (tid + n * NTH) / L::CH, i = magic ? __umulhi(r, magic) : r;
+            off[n] = (i * s1 + (r - i * G) * s2 + piece_col(n, tid)) * (unsigned)sizeof(T);
         }
     }
-    // row_at(n, r): the address of tile row r = row[n], or nullptr
-    template <typename F> __device__ __forceinline__ void load(unsigned lds, int tid, int D, F &&row_at) {
-        const unsigned wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // rows < `rows` of the tile at `base`; skip[n] < 0: not this one (with `skips`)
+    __device__ __forceinline__ void load(const T *base, unsigned lds, int tid, int D, int rows, bool skips, const int (&skip)[N]) const {
+        const unsigned at = lds + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
+        if (TOTAL % NTH == 0 && D == DP && rows >= ROWS && !skips) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            if (row[n] < 0) continue;
-            const T *p = row_at(n, row[n]);
-            if (p && col[n] < D) dma16(p + col[n], lds + (wave * 64 + n * NTH) * 16);
+            for (int n = 0; n < N; ++n) dma16(base, off[n], at + n * NTH * 16);
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (piece_row(n, tid, D) < rows && (!skips || skip[n] >= 0)) dma16(base, off[n], at + n * NTH * 16);
         }
     }
 };
@@ -222,7 +241,7 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // Scores in base 2: x = log2(e) (z - slope |pos - j|), z = scale q.k or c tanh(scale q.k / c).  tanh(u) = 1 - 2 / (e^{2u} + 1): one exponential and
 // one reciprocal; absolute error 1e-7, i.e. 1e-7 c of a score.  cap_in = 2 log2(e) scale / c, cap_out = c log2(e).
 template <bool CAP> __device__ __forceinline__ float tanh_of(float raw, float cap_in) {
-    return 1.f - 2.f * __builtin_amdgcn_rcpf(exp2_hw(raw * cap_in) + 1.f);
+    return fmaf(-2.f, __builtin_amdgcn_rcpf(exp2_hw(raw * cap_in) + 1.f), 1.f);
 }
 
 // what a row may see: keys j <= lim (lengths, causal order and prefix in one number), document equal

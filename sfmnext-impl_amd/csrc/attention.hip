@@ -56,12 +56,14 @@ template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float v = CAP ? A.cap_out * tanh_of<CAP>(x[nb][r], A.cap_in) : x[nb][r] * A.scale_log2;
+                    // without the bias the cap's factor goes into the exponent's fma, as the scale does
+                    float v = CAP ? tanh_of<CAP>(x[nb][r], A.cap_in) : x[nb][r];
+                    if (BIAS) v = v * (CAP ? A.cap_out : A.scale_log2);
                     if (BIAS) v = fmaf(-slope, fabsf((float)(pos - (j0 + nb * 32 + (r & 3) + 8 * (r >> 2) + 4 * h))), v);
                     x[nb][r] = v;
                 }
         }
-        const float c = CAP || BIAS ? 1.f : A.scale_log2;
+        const float c = BIAS ? 1.f : CAP ? A.cap_out : A.scale_log2;
         if (part) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -163,24 +165,25 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
 
     const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
     const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
-    S st(tid);
-    const unsigned ok[2] = {lds_offset(lk[0]), lds_offset(lk[1])}, ov[2] = {lds_offset(lv[0]), lds_offset(lv[1])};
+    S sk, sv;
+    sk.aim(tid, (unsigned)A.ks[1]);
+    sv.aim(tid, (unsigned)A.vs[1]);
+    const unsigned ok = lds_offset(lk[0]), ov = lds_offset(lv[0]);
     // padding keys (a negative document) are not loaded: their documents are read a tile ahead of the DMA that goes by them
     int pd[S::N], sd = -1;
     auto peek = [&](int t) {
         if (!kdoc) return;
 #pragma unroll
-        for (int n = 0; n < S::N; ++n) pd[n] = t < t1 && st.row[n] >= 0 && t * KT + st.row[n] < len ? kdoc[t * KT + st.row[n]] : -1;
+        for (int n = 0; n < S::N; ++n) {
+            const int r = S::piece_row(n, tid, A.D);
+            pd[n] = t < t1 && r < len - t * KT ? kdoc[t * KT + r] : -1;
+        }
         sd = t < t1 && tid < KT && t * KT + tid < len ? kdoc[t * KT + tid] : -1;
     };
     auto fetch = [&](int t, int s) {
-        const int j0 = t * KT;
-        auto rows = [&](const T *base, int64_t stride) {
-            const T *p0 = base + j0 * stride;
-            return [=, &pd](int n, int r) -> const T * { return j0 + r < len && (!kdoc || pd[n] >= 0) ? p0 + r * stride : nullptr; };
-        };
-        st.load(ok[s], tid, A.D, rows(kbase, A.ks[1]));
-        st.load(ov[s], tid, A.D, rows(vbase, A.vs[1]));
+        const int64_t j0 = (int64_t)t * KT;
+        sk.load(kbase + j0 * A.ks[1], ok + s * S::BYTES, tid, A.D, len - t * KT, kdoc != nullptr, pd);
+        sv.load(vbase + j0 * A.vs[1], ov + s * S::BYTES, tid, A.D, len - t * KT, kdoc != nullptr, pd);
         if (kdoc && tid < KT) ld[s][tid] = sd;
     };
 
@@ -287,16 +290,21 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
     for (int ks = 0; ks < L::KS; ++ks) qf[ks] = L::mem_frag(qrow, ks, h, A.D, row.on);
     const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
     const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
-    S st(lane);
+    S sk, sv;
+    sk.aim(lane, (unsigned)A.ks[1]);
+    sv.aim(lane, (unsigned)A.vs[1]);
     const unsigned o0 = lds_offset(buf[wave]);
     auto fetch = [&](int t, int s) {
         const int j0 = t * 32;
-        auto rows = [&](const T *base, int64_t stride) {
-            const T *p0 = base + j0 * stride;
-            return [=](int, int r) -> const T * { return j0 + r < len && (!kdoc || kdoc[j0 + r] >= 0) ? p0 + r * stride : nullptr; };
-        };
-        st.load(o0 + s * 2 * S::BYTES, lane, A.D, rows(kbase, A.ks[1]));
-        st.load(o0 + (s * 2 + 1) * S::BYTES, lane, A.D, rows(vbase, A.vs[1]));
+        int pd[S::N];
+        if (kdoc)
+#pragma unroll
+            for (int n = 0; n < S::N; ++n) {
+                const int r = S::piece_row(n, lane, A.D);
+                pd[n] = r < len - j0 ? kdoc[j0 + r] : -1;
+            }
+        sk.load(kbase + (int64_t)j0 * A.ks[1], o0 + s * 2 * S::BYTES, lane, A.D, len - j0, kdoc != nullptr, pd);
+        sv.load(vbase + (int64_t)j0 * A.vs[1], o0 + (s * 2 + 1) * S::BYTES, lane, A.D, len - j0, kdoc != nullptr, pd);
     };
     const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * 1.44269504088896341f : 0.f;
     Softmax<T, DP, 1, CAP, BIAS> sm;
@@ -430,6 +438,8 @@ int attn_check(const char *who, const sqd_attn_args *a) {
 }
 int attn_check_tensor(const char *who, const char *name, const void *p, const int64_t *stride, int dtype) {
     const int V = dtype == SQD_F32 ? 4 : 8;
+    SQD_CHECK_ARG(stride[1] >= 0 && stride[1] < (1 << 22) && stride[2] >= 0 && stride[2] < (1 << 22), "%s: token / head strides of %s: %lld, %lld", who, name,
+                  (long long)stride[1], (long long)stride[2]);
     SQD_CHECK_ARG(p && aligned16(p) && stride[0] % V == 0 && stride[1] % V == 0 && stride[2] % V == 0, "%s: %s must be 16-byte aligned, its strides too", who, name);
     return SQD_OK;
 }

@@ -25,19 +25,19 @@ using namespace sqd;
 constexpr int NT = 256, BM = 128;
 constexpr float ONE_LESS = 1.f - 2.384185791015625e-7f;        // 1 - 2^-22
 
-// delta [B,Hkv,Sq*G] (packed rows): 16 lanes a row, 8 features a lane.  o's rounding alone would be as large an error of a gradient as the rounding
-// of dS, so what it left (o_low) is added back.
+// What the two gradient kernels read of a packed row, padded to whole tiles: lse, delta = o.go, the last key it may see (-1: none, and then
+// its q and go are never loaded), document, and with a bias position and slope.  16 lanes a row, 8 features a lane.  o's rounding alone would be
+// as large an error of a gradient as the rounding of dS, so what it left (o_low) is added back.
 template <typename T>
-__global__ __launch_bounds__(NT) void attn_delta_kernel(AttnK A) {
-    const int RT = A.Sq * A.G, c = (threadIdx.x & 15) * 8;
-    const int64_t at = (int64_t)blockIdx.x * (NT / 16) + (threadIdx.x >> 4), rows = (int64_t)A.B * A.Hkv * RT;
-    if (at >= rows) return;
-    const int64_t bh = at / RT;
-    const int R = (int)(at - bh * RT), i = div_g(R, A.g_magic), hq = (int)(bh % A.Hkv) * A.G + R - i * A.G;
-    const int64_t b = bh / A.Hkv;
+__global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
+    const int RT = A.Sq * A.G, c = (threadIdx.x & 15) * 8, hk = blockIdx.y, b = blockIdx.z;
+    const int R = blockIdx.x * (NT / 16) + (threadIdx.x >> 4);
+    const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
+    const RowOf row = row_of(A, b, R, RT, len, A.prefix ? A.prefix[b] : 0);
+    const int hq = hk * A.G + row.g;
     float s = 0.f;
-    if (c < A.D) {
-        const int64_t o = ((b * A.Sq + i) * A.Hq + hq) * A.D + c;
+    if (c < A.D && row.lim >= 0) {
+        const int64_t o = (((int64_t)b * A.Sq + row.i) * A.Hq + hq) * A.D + c;
         float u[8], v[8];
         load_f32<T, 8>((const T *)A.o + o, u);
         if (sizeof(T) == 2 && A.o_low) {
@@ -45,29 +45,34 @@ __global__ __launch_bounds__(NT) void attn_delta_kernel(AttnK A) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[e] += v[e];
         }
-        load_f32<T, 8>((const T *)A.go + b * A.gos[0] + i * A.gos[1] + hq * A.gos[2] + c, v);
+        load_f32<T, 8>((const T *)A.go + b * A.gos[0] + (int64_t)row.i * A.gos[1] + hq * A.gos[2] + c, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s = fmaf(u[e], v[e], s);
     }
 #pragma unroll
     for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 16);
-    if ((threadIdx.x & 15) == 0) A.delta[at] = s;
+    if ((threadIdx.x & 15) == 0) {
+        const int64_t bh = (int64_t)b * A.Hkv + hk, at = bh * A.rows_padded + R;
+        A.row_delta[at] = s;
+        A.row_lse[at] = row.lim >= 0 ? A.lse[bh * RT + R] : INFINITY;
+        A.row_lim[at] = row.lim;
+        A.row_doc[at] = row.qd;
+        if (A.slopes) {
+            A.row_pos[at] = row.pos;
+            A.row_slope[at] = A.slopes[hq] * 1.44269504088896341f;
+        }
+    }
 }
 
-// probability and score gradient (without the scale) of one pair; `see` false: zeros, whatever the products hold
+// probability and score gradient (without the scale) of one pair, e = dP - delta; `see` false: zeros, whatever the products hold
 template <bool CAP, bool BIAS>
-__device__ __forceinline__ void pair_grad(float raw, float dp, float lse, float delta, float slope, float dist, const AttnK &A, bool see, float &p, float &ds) {
-    float x = raw, fac = 1.f;
-    if (CAP) {
-        const float t = tanh_of<CAP>(raw, A.cap_in);
-        fac = fmaf(-t, t, 1.f);
-        x = A.cap_out * t;
-    }
-    if (BIAS) x = fmaf(-slope, fabsf(dist), CAP ? x : x * A.scale_log2);
-    p = exp2_hw(fmaf(x, CAP || BIAS ? 1.f : A.scale_log2, -lse));
+__device__ __forceinline__ void pair_grad(float raw, float e, float lse, float slope, float dist, const AttnK &A, bool see, float &p, float &ds) {
+    const float t = CAP ? tanh_of<CAP>(raw, A.cap_in) : raw, c = CAP ? A.cap_out : A.scale_log2;
+    p = exp2_hw(BIAS ? fmaf(-slope, fabsf(dist), t * c) - lse : fmaf(t, c, -lse));
     p = see ? p : 0.f;
-    const float q = see && p < ONE_LESS ? p : 0.f, e = see ? dp - delta : 0.f;
-    ds = CAP ? q * e * fac : q * e;
+    const float q = see && p < ONE_LESS ? p : 0.f;
+    e = see ? e : 0.f;
+    ds = CAP ? q * e * fmaf(-t, t, 1.f) : q * e;
 }
 
 // 4 waves: KW of them side by side on 32 keys each, 4 / KW on the halves of a row tile.
@@ -78,8 +83,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
     typedef typename L::frag frag;
     typedef Stage<T, DP, QT, NT> S;
     __shared__ __align__(16) char lq[2][S::BYTES], lg[2][S::BYTES];
-    __shared__ __align__(16) float r_lse[2][QT], r_delta[2][QT], r_slope[2][QT];
-    __shared__ __align__(16) int r_lim[2][QT], r_doc[2][QT], r_pos[2][QT];
+    __shared__ __align__(16) float rows[2][6 * QT];            // lse, delta, last key, document; with a bias position, slope
     __shared__ int wk[8];
     static_assert(QW == 1 || sizeof(lq) >= (size_t)KW * (QW - 1) * 64 * DB * 16 * 4, "a wave's sums fit the row buffers");
 
@@ -131,50 +135,35 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
     }
 
     const T *qb = (const T *)A.q + b * A.qs[0] + (int64_t)hk * A.G * A.qs[2], *gb = (const T *)A.go + b * A.gos[0] + (int64_t)hk * A.G * A.gos[2];
-    S st(tid);
-    const unsigned oq[2] = {lds_offset(lq[0]), lds_offset(lq[1])}, og[2] = {lds_offset(lg[0]), lds_offset(lg[1])};
-    float s_lse = 0.f, s_delta = 0.f, s_slope = 0.f;
-    int s_lim = -1, s_doc = -2, s_pos = 0, s_i = 0;
-    // rows that see no key hold anything and are not loaded: documents are read a tile ahead of the DMA that goes by them
+    const int64_t row_at = (int64_t)bh * A.rows_padded;
+    S sq, sg;
+    sq.aim_packed(tid, 0, A.G, A.g_magic, (unsigned)A.qs[1], (unsigned)A.qs[2]);
+    sg.aim_packed(tid, 0, A.G, A.g_magic, (unsigned)A.gos[1], (unsigned)A.gos[2]);
+    const unsigned oq = lds_offset(lq[0]), og = lds_offset(lg[0]), orow = lds_offset(rows[0]);
+    // rows that see no key hold anything and are not loaded: their limits are read a tile ahead of the DMA that goes by them
+    const bool skips = docs || (A.causal && off < 0 && prefix <= 0);
     int pd[S::N];
     auto peek = [&](int t) {
-        if (!docs) return;
+        if (!skips) return;
 #pragma unroll
         for (int n = 0; n < S::N; ++n) {
-            const int R = t * QT + st.row[n];
-            pd[n] = t < nt && st.row[n] >= 0 && R < RT ? qdoc[div_g(R, A.g_magic)] : -1;
+            const int r = S::piece_row(n, tid, A.D);
+            pd[n] = t < nt && r < RT - t * QT ? A.row_lim[row_at + t * QT + r] : -1;
         }
-        const int R = t * QT + tid;
-        s_doc = t < nt && tid < QT && R < RT ? qdoc[div_g(R, A.g_magic)] : -2;
     };
     auto fetch = [&](int t, int s) {
-        auto rows = [&](const T *base, int64_t s1, int64_t s2) {
-            return [=, &A, &pd](int n, int r) -> const T * {
-                const int R = t * QT + r, i = div_g(R, A.g_magic);
-                if (R >= RT || (docs && pd[n] < 0) || row_limit(i + off, len, A.causal, prefix) < 0) return nullptr;
-                return base + i * s1 + (R - i * A.G) * s2;
-            };
-        };
-        if (tid < QT) {
-            const int R = t * QT + tid;
-            s_lim = -1, s_lse = INFINITY, s_delta = 0.f;
-            if (R < RT) {
-                s_i = div_g(R, A.g_magic);
-                s_pos = s_i + off;
-                s_lse = A.lse[(int64_t)bh * RT + R];
-                s_delta = A.delta[(int64_t)bh * RT + R];
-                if (BIAS) s_slope = A.slopes[hk * A.G + R - s_i * A.G] * 1.44269504088896341f;
-                if (!docs || s_doc >= 0) s_lim = row_limit(s_pos, len, A.causal, prefix);
-            }
-            if (docs) r_doc[s][tid] = s_doc;
+        const int i0 = div_g(t * QT, A.g_magic), rem = t * QT - i0 * A.G;
+        if (QT % A.G) {                                        // otherwise a tile starts with head 0 and the offsets are those of the first tile
+            sq.aim_packed(tid, rem, A.G, A.g_magic, (unsigned)A.qs[1], (unsigned)A.qs[2]);
+            sg.aim_packed(tid, rem, A.G, A.g_magic, (unsigned)A.gos[1], (unsigned)A.gos[2]);
         }
-        st.load(oq[s], tid, A.D, rows(qb, A.qs[1], A.qs[2]));
-        st.load(og[s], tid, A.D, rows(gb, A.gos[1], A.gos[2]));
-    };
-    auto put = [&](int s) {
-        if (tid < QT) {
-            r_lse[s][tid] = s_lse, r_delta[s][tid] = s_delta, r_lim[s][tid] = s_lim;
-            if (BIAS) r_slope[s][tid] = s_slope, r_pos[s][tid] = s_pos;
+        sq.load(qb + i0 * A.qs[1], oq + s * S::BYTES, tid, A.D, RT - t * QT, skips, pd);
+        sg.load(gb + i0 * A.gos[1], og + s * S::BYTES, tid, A.D, RT - t * QT, skips, pd);
+        if (wave == 3) {                                       // QT / 4 lanes an array
+            const int k = lane / (QT / 4), e = lane % (QT / 4) * 16;
+            const int64_t d1 = (const char *)A.row_delta - (const char *)A.row_lse;              // the arrays follow each other, d1 bytes apart
+            if (k < 4) dma16(A.row_lse + row_at + t * QT, (unsigned)(k * d1) + e, orow + s * 24 * QT);
+            if (BIAS && k < 2) dma16(A.row_pos + row_at + t * QT, (unsigned)(k * d1) + e, orow + s * 24 * QT + 16 * QT);
         }
     };
 
@@ -185,10 +174,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
     bool u, un;
     int t = walk.next(t0, u);
     peek(t);
-    if (t < nt) {
-        fetch(t, 0);
-        put(0);
-    }
+    if (t < nt) fetch(t, 0);
     int tn = walk.next(t + 1, un);
     peek(tn);
     dma_wait();
@@ -199,7 +185,14 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
         const int t2 = walk.next(tn + 1, u2);
         peek(t2);
         const int q0 = qw * 32;
-        f32x16 x = {}, dp = {};
+        const float *rw = rows[s];
+        f32x16 x = {}, dp;                                     // dp starts from -delta
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 d = *reinterpret_cast<const f32x4 *>(rw + QT + q0 + 8 * r4 + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * r4 + e] = -d[e];
+        }
 #pragma unroll
         for (int ks = 0; ks < L::KS; ++ks) {
             x = Mma<T>::mma(L::row_frag(lq[s], q0 + (lane & 31), ks, h), kf[ks], x);
@@ -213,18 +206,18 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int q4 = q0 + 8 * r4 + 4 * h;
-                const f32x4 lse = *reinterpret_cast<const f32x4 *>(&r_lse[s][q4]), delta = *reinterpret_cast<const f32x4 *>(&r_delta[s][q4]);
+                const f32x4 lse = *reinterpret_cast<const f32x4 *>(rw + q4);
                 int4 lim = make_int4(0, 0, 0, 0), qd = make_int4(kd, kd, kd, kd), ps = make_int4(0, 0, 0, 0);
                 f32x4 sl = {0, 0, 0, 0};
-                if (masked) lim = *reinterpret_cast<const int4 *>(&r_lim[s][q4]);
-                if (masked && docs) qd = *reinterpret_cast<const int4 *>(&r_doc[s][q4]);
-                if (BIAS) ps = *reinterpret_cast<const int4 *>(&r_pos[s][q4]), sl = *reinterpret_cast<const f32x4 *>(&r_slope[s][q4]);
+                if (masked) lim = *reinterpret_cast<const int4 *>(rw + 2 * QT + q4);
+                if (masked && docs) qd = *reinterpret_cast<const int4 *>(rw + 3 * QT + q4);
+                if (BIAS) ps = *reinterpret_cast<const int4 *>(rw + 4 * QT + q4), sl = *reinterpret_cast<const f32x4 *>(rw + 5 * QT + q4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e;
                     const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
                     const int pe = e == 0 ? ps.x : e == 1 ? ps.y : e == 2 ? ps.z : ps.w;
-                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], delta[e], sl[e], (float)(pe - jl), A, !masked || (jl <= le && de == kd), p[r], ds[r]);
+                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], sl[e], (float)(pe - jl), A, !masked || (jl <= le && de == kd), p[r], ds[r]);
                 }
             }
         };
@@ -239,7 +232,6 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
                 gk[db] = Mma<T>::mma(L::col_frag(lq[s], q0 + kk * 16, db, lane), df, gk[db]);
             }
         }
-        if (tn < nt) put(s ^ 1);
         dma_wait();
         __syncthreads();
         s ^= 1;
@@ -332,27 +324,28 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         gf[ks] = L::mem_frag(grow, ks, h, A.D, live);
     }
     float lse = INFINITY, delta = 0.f;
-    if (live) lse = A.lse[(int64_t)bh * RT + R], delta = A.delta[(int64_t)bh * RT + R];
+    if (live) lse = A.row_lse[(int64_t)bh * A.rows_padded + R], delta = A.row_delta[(int64_t)bh * A.rows_padded + R];
 
     const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
     const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
-    S st(tid);
-    const unsigned ok[2] = {lds_offset(lk[0]), lds_offset(lk[1])}, ov[2] = {lds_offset(lv[0]), lds_offset(lv[1])};
+    S sk, sv;
+    sk.aim(tid, (unsigned)A.ks[1]);
+    sv.aim(tid, (unsigned)A.vs[1]);
+    const unsigned ok = lds_offset(lk[0]), ov = lds_offset(lv[0]);
     int pd[S::N], sd = -1;                                     // as in the forward
     auto peek = [&](int t) {
         if (!kdoc) return;
 #pragma unroll
-        for (int n = 0; n < S::N; ++n) pd[n] = t < t1 && st.row[n] >= 0 && t * KT + st.row[n] < len ? kdoc[t * KT + st.row[n]] : -1;
+        for (int n = 0; n < S::N; ++n) {
+            const int r = S::piece_row(n, tid, A.D);
+            pd[n] = t < t1 && r < len - t * KT ? kdoc[t * KT + r] : -1;
+        }
         sd = t < t1 && tid < KT && t * KT + tid < len ? kdoc[t * KT + tid] : -1;
     };
     auto fetch = [&](int t, int s) {
-        const int j0 = t * KT;
-        auto rows = [&](const T *base, int64_t stride) {
-            const T *p0 = base + j0 * stride;
-            return [=, &pd](int n, int r) -> const T * { return j0 + r < len && (!kdoc || pd[n] >= 0) ? p0 + r * stride : nullptr; };
-        };
-        st.load(ok[s], tid, A.D, rows(kbase, A.ks[1]));
-        st.load(ov[s], tid, A.D, rows(vbase, A.vs[1]));
+        const int64_t j0 = (int64_t)t * KT;
+        sk.load(kbase + j0 * A.ks[1], ok + s * S::BYTES, tid, A.D, len - t * KT, kdoc != nullptr, pd);
+        sv.load(vbase + j0 * A.vs[1], ov + s * S::BYTES, tid, A.D, len - t * KT, kdoc != nullptr, pd);
         if (kdoc && tid < KT) ld[s][tid] = sd;
     };
     const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * 1.44269504088896341f : 0.f;
@@ -393,7 +386,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
                     float p;
-                    pair_grad<CAP, BIAS>(x[r], dp[r], lse, delta, slope, (float)(row.pos - j), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
+                    pair_grad<CAP, BIAS>(x[r], dp[r] - delta, lse, slope, (float)(row.pos - j), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
                 }
             }
         };
@@ -422,27 +415,25 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         }
 }
 
-struct BwdPlan { int64_t rows; int kw, nq_tiles, nk_tiles; int64_t delta, q_rng, k_rng; };
+struct BwdPlan { int kw, rows_padded, nq_tiles, nk_tiles; int64_t rows, scratch; };
 BwdPlan bwd_plan(const sqd_attn_args *a) {
     BwdPlan p{};
     const int G = a->Hq / a->Hkv;
-    p.rows = (int64_t)a->B * a->Hkv * a->Sq * G;
     // keys a workgroup: 128, or 64 with the row tile split between the waves while 128 would leave CUs idle or a last round nearly empty
     p.kw = (int64_t)((a->Sk + 127) / 128) * a->B * a->Hkv < 1024 ? 2 : 4;
     const int QT = 32 * (4 / p.kw);
+    p.rows_padded = (a->Sq * G + 63) / 64 * 64;
+    p.rows = (int64_t)a->B * a->Hkv * p.rows_padded;
     p.nq_tiles = a->q_docs ? (a->Sq * G + QT - 1) / QT : 0;
     p.nk_tiles = a->q_docs ? (a->Sk + 31) / 32 : 0;
-    p.delta = (p.rows + 3) / 4 * 4;
-    p.q_rng = (int64_t)2 * a->B * p.nq_tiles;
-    p.k_rng = (int64_t)2 * a->B * p.nk_tiles;
+    p.scratch = (a->slopes ? 6 : 4) * p.rows + (int64_t)2 * a->B * (p.nq_tiles + p.nk_tiles);
     return p;
 }
 }  // namespace
 
 extern "C" int64_t sqd_attn_bwd_scratch(const sqd_attn_args *a) {
     if (sqd::attn_check("sqd_attn_bwd_scratch", a)) return SQD_EINVAL;
-    const BwdPlan p = bwd_plan(a);
-    return p.delta + p.q_rng + p.k_rng;
+    return bwd_plan(a).scratch;
 }
 
 extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
@@ -453,7 +444,8 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
     if (a->Sq) {
         if (int e = attn_check_tensor(who, "q", a->q, a->q_stride, a->dtype)) return e;
         if (int e = attn_check_tensor(who, "go", a->go, a->go_stride, a->dtype)) return e;
-        SQD_CHECK_ARG(a->o && aligned16(a->o) && a->gq && aligned16(a->gq) && a->lse && a->scratch && aligned16(a->scratch), "%s: null or unaligned pointer", who);
+        SQD_CHECK_ARG(a->o && aligned16(a->o) && aligned16(a->o_low) && a->gq && aligned16(a->gq) && a->lse && a->scratch && aligned16(a->scratch),
+                      "%s: null or unaligned pointer", who);
     }
     if (a->Sk) {
         if (int e = attn_check_tensor(who, "k", a->k, a->k_stride, a->dtype)) return e;
@@ -461,13 +453,17 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
         SQD_CHECK_ARG(a->gk && a->gv && aligned16(a->gk) && aligned16(a->gv), "%s: null or unaligned pointer", who);
     }
     const BwdPlan p = bwd_plan(a);
+    SQD_CHECK_ARG(p.rows < (1 << 28) && a->B < 65536 && a->Hkv < 65536, "%s: too many tokens", who);          // row records: 32-bit offsets between arrays
     AttnK A = attn_kargs(a);
-    A.delta = a->scratch;
-    int2 *q_rng = reinterpret_cast<int2 *>(a->scratch + p.delta), *k_rng = q_rng + (int64_t)a->B * p.nq_tiles;
+    A.rows_padded = p.rows_padded;
+    A.row_lse = a->scratch, A.row_delta = a->scratch + p.rows;
+    A.row_lim = (int *)(a->scratch + 2 * p.rows), A.row_doc = (int *)(a->scratch + 3 * p.rows);
+    A.row_pos = (int *)(a->scratch + 4 * p.rows), A.row_slope = a->scratch + 5 * p.rows;
+    int2 *q_rng = reinterpret_cast<int2 *>(a->scratch + (a->slopes ? 6 : 4) * p.rows), *k_rng = q_rng + (int64_t)a->B * p.nq_tiles;
     const hipStream_t st = (hipStream_t)a->stream;
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);
-        if (p.rows) hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((p.rows + 15) / 16)), dim3(NT), 0, st, A);
+        if (p.rows) hipLaunchKernelGGL((attn_rows_kernel<T>), dim3(p.rows_padded / 16, A.Hkv, A.B), dim3(NT), 0, st, A);
         if (p.nq_tiles) attn_doc_ranges(A.q_docs, q_rng, A.B, A.Sq, A.G, 32 * (4 / p.kw), p.nq_tiles, st);
         if (p.nk_tiles) attn_doc_ranges(A.k_docs, k_rng, A.B, A.Sk, 1, 32, p.nk_tiles, st);
         auto go = [&](auto dp, auto cap, auto bias) {

@@ -21,20 +21,22 @@ def on_device(t):
 
 
 def _rows16(t):
-    """t with features dense and every other stride and the address in whole 16-byte pieces: itself, or a copy"""
+    """t [B,S,H,D] with features dense, every other stride and the address in whole 16-byte pieces and the strides of tokens and heads below
+    2^22 elements: itself, or a copy"""
     n = 16 // t.element_size()
     if t.numel() == 0:
         return t
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % n == 0 for s, d in zip(t.stride()[:-1], t.shape[:-1]) if d > 1):
+    (b, s, h, e), (B, S, H, _) = t.stride(), t.shape
+    if (e == 1 and t.data_ptr() % 16 == 0 and (B == 1 or b % n == 0) and (S == 1 or (s % n == 0 and 0 <= s < 1 << 22))
+            and (H == 1 or (h % n == 0 and 0 <= h < 1 << 22))):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t):
-    """element strides of batch, token and head; a dimension of one element counts as dense"""
-    n = 16 // t.element_size()
-    return [s if d > 1 else n * (s // n) for s, d in zip(t.stride()[:3], t.shape[:3])]
+    """element strides of batch, token and head; 0 where there is one only"""
+    return [s if d > 1 else 0 for s, d in zip(t.stride()[:3], t.shape[:3])]
 
 
 # ------------------------------------------------------------------------------------------------------------------ residual RMS norm
