@@ -138,7 +138,13 @@ template <typename T, int DP> struct Tile {
 __device__ __forceinline__ void dma16(const void *base, unsigned off, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// (the builtin and not assembly: the compiler then knows that its own earlier loads have arrived too, and does not wait for them, and with
+// them for a DMA under way, in the middle of a loop)
+__device__ __forceinline__ void dma_wait() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);                         // vmcnt(0)
+    asm volatile("" ::: "memory");
+}
 __device__ __forceinline__ unsigned lds_offset(const void *p) {
     return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)p);
 }
@@ -186,6 +192,34 @@ template <typename T, int DP, int ROWS, int NTH> struct Stage {
         }
     }
 };
+
+// acc[n] += sum over the features of frag_a(n, ks) x b[ks]: the LDS reads of BATCH steps are in flight while the step before multiplies.  Left to
+// itself the compiler reads one operand, waits for it and multiplies, and the LDS latency (some 130 cycles, against 32 of the product)
+// is paid in every step; the scheduling barriers keep the batches apart.
+template <typename T, int NACC, int KS, typename F>
+__device__ __forceinline__ void product(f32x16 (&acc)[NACC], const typename Mma<T>::frag (&b)[KS], F &&frag_a) {
+    constexpr int BATCH = sizeof(T) == 4 ? (KS < 2 ? KS : 2) : (KS < 4 ? KS : 4), STEPS = NACC * KS / BATCH;
+    typename Mma<T>::frag f[2][BATCH];
+    auto fetch = [&](auto st) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int u = decltype(st)::value * BATCH + i;
+            f[decltype(st)::value & 1][i] = frag_a(u / KS, u % KS);
+        }
+    };
+    fetch(std::integral_constant<int, 0>{});
+    static_for<STEPS>([&](auto st) {
+        constexpr int S = decltype(st)::value;
+        if constexpr (S + 1 < STEPS) fetch(std::integral_constant<int, S + 1>{});
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int u = S * BATCH + i;
+            acc[u / KS] = Mma<T>::mma(f[S & 1][i], b[u % KS], acc[u / KS]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    });
+}
 
 // zeros over `bytes` (a multiple of 16) of LDS by NTH threads
 template <int NTH> __device__ __forceinline__ void clear_lds(char *p, int bytes, int tid) {

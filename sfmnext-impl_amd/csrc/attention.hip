@@ -95,21 +95,27 @@ template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
             m = mn;
         }
         const float base = m == -INFINITY ? 0.f : m;
+        // 16 keys at a time: their values' operands are read while the step before multiplies, and the exponentials of a step run under its products
+        typename L::frag vf[2][DB];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int db = 0; db < DB; ++db) vf[0][db] = L::col_frag(lv, 0, db, lane);
+        static_for<2 * NB>([&](auto step) {
+            constexpr int K = decltype(step)::value;
+            float p[8];
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                float p[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    p[r] = exp2_hw(fmaf(x[nb][8 * kk + r], c, -base));
-                    l += p[r];
-                }
-                // P is rounded to the values' type for the second product (half a step of that type, relative); the sum keeps the unrounded P
-                const typename L::frag pf = Mma<T>::pack(p);
-#pragma unroll
-                for (int db = 0; db < DB; ++db) o[db] = Mma<T>::mma(L::col_frag(lv, nb * 32 + kk * 16, db, lane), pf, o[db]);
+            for (int r = 0; r < 8; ++r) {
+                p[r] = exp2_hw(fmaf(x[K / 2][8 * (K & 1) + r], c, -base));
+                l += p[r];
             }
+            // P is rounded to the values' type for the second product (half a step of that type, relative); the sum keeps the unrounded P
+            const typename L::frag pf = Mma<T>::pack(p);
+            if constexpr (K + 1 < 2 * NB)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) vf[(K + 1) & 1][db] = L::col_frag(lv, (K + 1) * 16, db, lane);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[db] = Mma<T>::mma(vf[K & 1][db], pf, o[db]);
+        });
     }
 };
 
@@ -205,11 +211,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         peek(t2);
         f32x16 x[NB];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            x[nb] = f32x16{};
-#pragma unroll
-            for (int ks = 0; ks < L::KS; ++ks) x[nb] = Mma<T>::mma(L::row_frag(lk[s], nb * 32 + (lane & 31), ks, h), qf[ks], x[nb]);
-        }
+        for (int nb = 0; nb < NB; ++nb) x[nb] = f32x16{};
+        product<T>(x, qf, [&](int nb, int ks) { return L::row_frag(lk[s], nb * 32 + (lane & 31), ks, h); });
         // the mask, where a row of the wave does not see the whole tile
         const bool part = !u || __any(row.lim < t * KT + KT - 1);
         sm.tile(x, A, lv[s], ld[s], kdoc != nullptr, part, t * KT, row.pos, row.lim, row.qd, slope, lane);
@@ -317,8 +320,7 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
         if (kdoc && lane < 32) ld[wave][lane] = j0 + lane < len ? kdoc[j0 + lane] : -1;
         const char *lk = buf[wave] + s * 2 * S::BYTES, *lv = lk + S::BYTES;
         f32x16 x[1] = {f32x16{}};
-#pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks) x[0] = Mma<T>::mma(L::row_frag(lk, lane & 31, ks, h), qf[ks], x[0]);
+        product<T>(x, qf, [&](int, int ks) { return L::row_frag(lk, lane & 31, ks, h); });
         const bool part = kdoc != nullptr || __any(row.lim < j0 + 31);
         sm.tile(x, A, lv, ld[wave], kdoc != nullptr, part, j0, row.pos, row.lim, row.qd, slope, lane);
         t += NW;

@@ -186,18 +186,16 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
         peek(t2);
         const int q0 = qw * 32;
         const float *rw = rows[s];
-        f32x16 x = {}, dp;                                     // dp starts from -delta
+        f32x16 xs[1] = {f32x16{}}, dps[1];                     // dP starts from -delta
+        f32x16 &x = xs[0], &dp = dps[0];
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
             const f32x4 d = *reinterpret_cast<const f32x4 *>(rw + QT + q0 + 8 * r4 + 4 * h);
 #pragma unroll
             for (int e = 0; e < 4; ++e) dp[4 * r4 + e] = -d[e];
         }
-#pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks) {
-            x = Mma<T>::mma(L::row_frag(lq[s], q0 + (lane & 31), ks, h), kf[ks], x);
-            dp = Mma<T>::mma(L::row_frag(lg[s], q0 + (lane & 31), ks, h), vf[ks], dp);
-        }
+        product<T>(xs, kf, [&](int, int ks) { return L::row_frag(lq[s], q0 + (lane & 31), ks, h); });
+        product<T>(dps, vf, [&](int, int ks) { return L::row_frag(lg[s], q0 + (lane & 31), ks, h); });
         // every row of the tile sees all of the wave's keys?  (limits do not fall with the row)
         const int R0 = t * QT + q0;
         const bool part = !all_on || !u || R0 + 32 > RT || row_limit(div_g(R0, A.g_magic) + off, len, A.causal, prefix) < j0 + kw * 32 + 31;
@@ -223,15 +221,24 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
         };
         if (part) grads(std::true_type{});
         else grads(std::false_type{});
+        // gV, gK for 16 rows, then for the other 16; the operands of a step are read while the step before multiplies
+        frag cf[2][DB];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const frag pf = Mma<T>::pack(&p[8 * kk]), df = Mma<T>::pack(&ds[8 * kk]);
+        for (int db = 0; db < DB; ++db) cf[0][db] = L::col_frag(lg[s], q0, db, lane);
+        static_for<4>([&](auto step) {
+            constexpr int K = decltype(step)::value;
+            const frag f = Mma<T>::pack((K & 1 ? ds : p) + 8 * (K / 2));
+            if constexpr (K < 3)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) cf[(K + 1) & 1][db] = L::col_frag(K & 1 ? lg[s] : lq[s], q0 + (K + 1) / 2 * 16, db, lane);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                gv[db] = Mma<T>::mma(L::col_frag(lg[s], q0 + kk * 16, db, lane), pf, gv[db]);
-                gk[db] = Mma<T>::mma(L::col_frag(lq[s], q0 + kk * 16, db, lane), df, gk[db]);
+                f32x16 &g = (K & 1 ? gk : gv)[db];
+                g = Mma<T>::mma(cf[K & 1][db], f, g);
             }
-        }
+            __builtin_amdgcn_sched_barrier(0);
+        });
         dma_wait();
         __syncthreads();
         s ^= 1;
@@ -368,12 +375,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         const int t2 = walk.next(tn + 1, u2);
         peek(t2);
         const int j0 = t * KT;
-        f32x16 x = {}, dp = {};
-#pragma unroll
-        for (int ks = 0; ks < L::KS; ++ks) {
-            x = Mma<T>::mma(L::row_frag(lk[s], lane & 31, ks, h), qf[ks], x);
-            dp = Mma<T>::mma(L::row_frag(lv[s], lane & 31, ks, h), gf[ks], dp);
-        }
+        f32x16 xs[1] = {f32x16{}}, dps[1] = {f32x16{}};
+        f32x16 &x = xs[0], &dp = dps[0];
+        product<T>(xs, qf, [&](int, int ks) { return L::row_frag(lk[s], lane & 31, ks, h); });
+        product<T>(dps, gf, [&](int, int ks) { return L::row_frag(lv[s], lane & 31, ks, h); });
         const bool part = !u || __any(row.lim < j0 + KT - 1);
         float ds[16];
         auto grads = [&](auto masked) {
@@ -392,11 +397,17 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         };
         if (part) grads(std::true_type{});
         else grads(std::false_type{});
+        frag cf[2][DB];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) cf[kk][db] = L::col_frag(lk[s], kk * 16, db, lane);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             const frag df = Mma<T>::pack(&ds[8 * kk]);
 #pragma unroll
-            for (int db = 0; db < DB; ++db) gq[db] = Mma<T>::mma(L::col_frag(lk[s], kk * 16, db, lane), df, gq[db]);
+            for (int db = 0; db < DB; ++db) gq[db] = Mma<T>::mma(cf[kk][db], df, gq[db]);
         }
         dma_wait();
         __syncthreads();
