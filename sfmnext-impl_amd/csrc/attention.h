@@ -20,18 +20,22 @@
 
 namespace sqd {
 
+struct Deal { int m, slots, share; };       // workgroups to tiles: see dealt()
+
 struct AttnK {
     const void *q, *k, *v, *go;
     void *o, *o_low, *gq, *gk, *gv;
     float *lse, *part_o, *part_lse;
-    float *row_lse, *row_delta, *row_slope;  // the backward's copies by packed row, padded to whole tiles (rows_padded a key head)
-    int *row_lim, *row_doc, *row_pos;
+    float *row_lse, *row_delta, *row_pos, *row_slope;  // the backward's copies by packed row, padded to whole tiles (rows_padded a key head)
+    int *row_lim, *row_doc;
     const float *slopes;
     const int *prefix, *q_docs, *k_docs, *k_len;
     const int2 *doc_rng;                    // per tile of the looped-over side: smallest and largest document id
     int64_t qs[3], ks[3], vs[3], gos[3];
     float scale_log2, cap_in, cap_out, scale;             // log2(e) scale; 2 log2(e) scale / cap, cap log2(e)
     unsigned g_magic;
+    Deal deal;
+    float unit_inv;                          // slopes are used in units of the raw score (1 / scale) or of tanh (1 / cap)
     int B, Sq, Sk, Hq, Hkv, G, D, causal, ntile, nsplit, ndoc_tiles, rows_padded;
 };
 
@@ -299,10 +303,23 @@ __device__ __forceinline__ RowOf row_of(const AttnK &A, int b, int R, int RT, in
     return r;
 }
 
-// n workgroups dealt to 8 XCDs round robin: workgroup id -> work item such that an XCD gets consecutive items (they share keys and values in
-// its L2)
-__device__ __forceinline__ int xcd_order(int id, int n) {
-    const int x = id & 7, k = id >> 3, base = n >> 3, more = n & 7;
-    return x * base + min(x, more) + k;
+// Workgroups are dealt to the 8 XCDs round robin; the ones that share keys and values (a group: one batch row's key head) belong on one XCD and its
+// L2.  With a number of groups that 8 does not divide a group is shared by m = 8 / gcd(8, groups) XCDs, its tiles dealt in turn: in causal
+// order the tiles' work grows along the group, and consecutive halves would be as 1 to 3 (8192 tokens, 4 groups: 410 us that way).
+// id -> group and tile, the last tile first; false: no such tile.
+inline Deal deal(int groups, int tiles) {
+    const int g = groups % 8 == 0 ? 8 : groups % 4 == 0 ? 4 : groups % 2 == 0 ? 2 : 1;
+    Deal d;
+    d.m = 8 / g;
+    d.slots = (tiles + d.m - 1) / d.m;
+    d.share = groups / g;                   // sub-groups an XCD takes
+    return d;
+}
+inline int64_t deal_blocks(const Deal &d) { return (int64_t)8 * d.share * d.slots; }
+__device__ __forceinline__ bool dealt(const Deal &d, int id, int tiles, int &group, int &tile) {
+    const int x = id & 7, k = id >> 3, local = k / d.slots, j = k - local * d.slots, sub = x * d.share + local;
+    group = sub / d.m;
+    tile = j * d.m + sub - group * d.m;
+    return tile < tiles;
 }
 }  // namespace sqd

@@ -51,19 +51,17 @@ template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
     __device__ __forceinline__ void tile(f32x16 (&x)[NB], const AttnK &A, const char *lv, const int *ld, bool docs, bool part, int j0, int pos, int lim, int qd,
                                          float slope, int lane) {
         const int h = lane >> 5;
+        // scores in units of c = log2(e) scale, or of c = log2(e) cap behind tanh: c goes into the exponent's fma
+        const float c = CAP ? A.cap_out : A.scale_log2, d0 = (float)(pos - j0 - 4 * h);
         if (CAP || BIAS) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    // without the bias the cap's factor goes into the exponent's fma, as the scale does
-                    float v = CAP ? tanh_of<CAP>(x[nb][r], A.cap_in) : x[nb][r];
-                    if (BIAS) v = v * (CAP ? A.cap_out : A.scale_log2);
-                    if (BIAS) v = fmaf(-slope, fabsf((float)(pos - (j0 + nb * 32 + (r & 3) + 8 * (r >> 2) + 4 * h))), v);
-                    x[nb][r] = v;
+                    if (CAP) x[nb][r] = tanh_of<CAP>(x[nb][r], A.cap_in);
+                    if (BIAS) x[nb][r] = fmaf(-slope, fabsf(d0 - (float)(nb * 32 + (r & 3) + 8 * (r >> 2))), x[nb][r]);
                 }
         }
-        const float c = BIAS ? 1.f : CAP ? A.cap_out : A.scale_log2;
         if (part) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -130,10 +128,9 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     __shared__ int wq[8];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    int w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = A.ntile - 1 - w % A.ntile;                 // the longest causal rows first
-    w /= A.ntile;
-    const int split = w % A.nsplit, bh = w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
+    int bh, w;
+    if (!dealt(A.deal, blockIdx.x, A.ntile * A.nsplit, bh, w)) return;
+    const int split = w % A.nsplit, tile = A.ntile - 1 - w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;        // the longest causal rows first
     const int RT = A.Sq * A.G, row0 = tile * BM;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
     const int prefix = A.prefix ? A.prefix[b] : 0;
@@ -193,7 +190,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         if (kdoc && tid < KT) ld[s][tid] = sd;
     };
 
-    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * 1.44269504088896341f : 0.f;
+    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * A.unit_inv : 0.f;
     Softmax<T, DP, NB, CAP, BIAS> sm;
     int s = 0;
     bool u, un;
@@ -266,8 +263,9 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
     __shared__ float wm[NW][32], wl[NW][32];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    int w = xcd_order(blockIdx.x, gridDim.x);
-    const int split = w % A.nsplit, bh = w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
+    int bh, split;
+    if (!dealt(A.deal, blockIdx.x, A.nsplit, bh, split)) return;
+    const int hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, R = lane & 31;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
     const int prefix = A.prefix ? A.prefix[b] : 0;
@@ -309,7 +307,7 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
         sk.load(kbase + (int64_t)j0 * A.ks[1], o0 + s * 2 * S::BYTES, lane, A.D, len - j0, kdoc != nullptr, pd);
         sv.load(vbase + (int64_t)j0 * A.vs[1], o0 + (s * 2 + 1) * S::BYTES, lane, A.D, len - j0, kdoc != nullptr, pd);
     };
-    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * 1.44269504088896341f : 0.f;
+    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * A.unit_inv : 0.f;
     Softmax<T, DP, 1, CAP, BIAS> sm;
     int t = t0 + wave, s = 0;
     if (t < t1) fetch(t, 0);
@@ -432,7 +430,7 @@ int attn_check(const char *who, const sqd_attn_args *a) {
     SQD_CHECK_ARG(a->D >= 8 && a->D <= 128 && a->D % 8 == 0, "%s: %d features a head (a multiple of 8 up to 128)", who, a->D);
     SQD_CHECK_ARG(a->Sk < (1 << 24) && (int64_t)a->Sq * (a->Hq / a->Hkv) < (1 << 30) &&
                       (int64_t)a->Sq * (a->Hq / a->Hkv) * (a->Hq / a->Hkv) < (1ll << 31) && (int64_t)a->B * a->Hkv < (1 << 24), "%s: too many tokens", who);
-    SQD_CHECK_ARG(a->scale > 0.f && a->scale < 3e38f && a->softcap >= 0.f && a->softcap < 3e38f, "%s: scale %g, cap %g", who, (double)a->scale, (double)a->softcap);
+    SQD_CHECK_ARG(a->scale > 1e-30f && a->scale < 1e30f && a->softcap >= 0.f && a->softcap < 1e30f && (a->softcap == 0.f || a->softcap > 1e-30f), "%s: scale %g, cap %g", who, (double)a->scale, (double)a->softcap);
     SQD_CHECK_ARG(a->dtype >= SQD_F32 && a->dtype <= SQD_F16, "%s: element type %d", who, a->dtype);
     SQD_CHECK_ARG(!a->prefix || a->causal, "%s: a prefix needs the causal order", who);
     SQD_CHECK_ARG(!a->q_docs == !a->k_docs, "%s: documents of queries and keys come together", who);
@@ -453,6 +451,7 @@ AttnK attn_kargs(const sqd_attn_args *a) {
     constexpr double LOG2E = 1.44269504088896340736;
     A.scale = a->scale;
     A.scale_log2 = (float)(a->scale * LOG2E);
+    A.unit_inv = (float)(1.0 / (a->softcap > 0.f ? a->softcap : a->scale));
     if (a->softcap > 0.f) A.cap_in = (float)(2.0 * LOG2E * a->scale / a->softcap), A.cap_out = (float)(a->softcap * LOG2E);
     A.B = a->B, A.Sq = a->Sq, A.Sk = a->Sk, A.Hq = a->Hq, A.Hkv = a->Hkv, A.G = a->Hq / a->Hkv, A.D = a->D, A.causal = a->causal;
     A.g_magic = A.G == 1 ? 0u : (unsigned)(((1ull << 32) + A.G - 1) / A.G);
@@ -487,7 +486,10 @@ extern "C" int sqd_attn_fwd(const sqd_attn_args *a) {
     A.part_o = a->scratch, A.part_lse = a->scratch + p.part_floats;
     int2 *rng = reinterpret_cast<int2 *>(a->scratch + p.part_floats + p.lse_floats);
     A.doc_rng = rng;
-    const int64_t blocks = (int64_t)A.ntile * A.nsplit * A.B * A.Hkv;
+    const int64_t tiles = (int64_t)A.ntile * A.nsplit;
+    SQD_CHECK_ARG(tiles < (1 << 24), "sqd_attn_fwd: too many tokens");
+    A.deal = deal(A.B * A.Hkv, (int)tiles);
+    const int64_t blocks = deal_blocks(A.deal);
     SQD_CHECK_ARG(blocks < (1ll << 31), "sqd_attn_fwd: too many tokens");
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);

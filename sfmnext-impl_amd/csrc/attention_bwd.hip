@@ -58,8 +58,8 @@ __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
         A.row_lim[at] = row.lim;
         A.row_doc[at] = row.qd;
         if (A.slopes) {
-            A.row_pos[at] = row.pos;
-            A.row_slope[at] = A.slopes[hq] * 1.44269504088896341f;
+            A.row_pos[at] = (float)row.pos;
+            A.row_slope[at] = A.slopes[hq] * A.unit_inv;
         }
     }
 }
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
 template <bool CAP, bool BIAS>
 __device__ __forceinline__ void pair_grad(float raw, float e, float lse, float slope, float dist, const AttnK &A, bool see, float &p, float &ds) {
     const float t = CAP ? tanh_of<CAP>(raw, A.cap_in) : raw, c = CAP ? A.cap_out : A.scale_log2;
-    p = exp2_hw(BIAS ? fmaf(-slope, fabsf(dist), t * c) - lse : fmaf(t, c, -lse));
+    p = exp2_hw(fmaf(BIAS ? fmaf(-slope, fabsf(dist), t) : t, c, -lse));
     p = see ? p : 0.f;
     const float q = see && p < ONE_LESS ? p : 0.f;
     e = see ? e : 0.f;
@@ -88,8 +88,9 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
     static_assert(QW == 1 || sizeof(lq) >= (size_t)KW * (QW - 1) * 64 * DB * 16 * 4, "a wave's sums fit the row buffers");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, kw = wave % KW, qw = wave / KW;
-    int w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = w % A.ntile, bh = w / A.ntile, hk = bh % A.Hkv, b = bh / A.Hkv;
+    int bh, tile;                                              // the first keys (the most rows, in causal order) first
+    if (!dealt(A.deal, blockIdx.x, A.ntile, bh, tile)) return;
+    const int hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, j0 = tile * 32 * KW, jl = j0 + kw * 32 + (lane & 31);
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk, off = len - A.Sq;
     const int prefix = A.prefix ? A.prefix[b] : 0;
@@ -124,6 +125,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
     if (j0 >= len) t0 = nt;
     DocWalk walk(docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, nt);
     const bool all_on = __all(on);
+    const float jf = (float)jl;
 
     frag kf[L::KS], vf[L::KS];
     const T *krow = (const T *)A.k + b * A.ks[0] + (int64_t)jl * A.ks[1] + hk * A.ks[2];
@@ -205,17 +207,16 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int q4 = q0 + 8 * r4 + 4 * h;
                 const f32x4 lse = *reinterpret_cast<const f32x4 *>(rw + q4);
-                int4 lim = make_int4(0, 0, 0, 0), qd = make_int4(kd, kd, kd, kd), ps = make_int4(0, 0, 0, 0);
-                f32x4 sl = {0, 0, 0, 0};
+                int4 lim = make_int4(0, 0, 0, 0), qd = make_int4(kd, kd, kd, kd);
+                f32x4 ps = {0, 0, 0, 0}, sl = {0, 0, 0, 0};
                 if (masked) lim = *reinterpret_cast<const int4 *>(rw + 2 * QT + q4);
                 if (masked && docs) qd = *reinterpret_cast<const int4 *>(rw + 3 * QT + q4);
-                if (BIAS) ps = *reinterpret_cast<const int4 *>(rw + 4 * QT + q4), sl = *reinterpret_cast<const f32x4 *>(rw + 5 * QT + q4);
+                if (BIAS) ps = *reinterpret_cast<const f32x4 *>(rw + 4 * QT + q4), sl = *reinterpret_cast<const f32x4 *>(rw + 5 * QT + q4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e;
                     const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
-                    const int pe = e == 0 ? ps.x : e == 1 ? ps.y : e == 2 ? ps.z : ps.w;
-                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], sl[e], (float)(pe - jl), A, !masked || (jl <= le && de == kd), p[r], ds[r]);
+                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), p[r], ds[r]);
                 }
             }
         };
@@ -292,8 +293,9 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     __shared__ int wq[8];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    int w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = A.ntile - 1 - w % A.ntile, bh = w / A.ntile, hk = bh % A.Hkv, b = bh / A.Hkv;
+    int bh, w;
+    if (!dealt(A.deal, blockIdx.x, A.ntile, bh, w)) return;
+    const int tile = A.ntile - 1 - w, hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, row0 = tile * BM;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
     const int prefix = A.prefix ? A.prefix[b] : 0;
@@ -355,7 +357,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         sv.load(vbase + j0 * A.vs[1], ov + s * S::BYTES, tid, A.D, len - t * KT, kdoc != nullptr, pd);
         if (kdoc && tid < KT) ld[s][tid] = sd;
     };
-    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * 1.44269504088896341f : 0.f;
+    const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * A.unit_inv : 0.f;
     f32x16 gq[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) gq[db] = f32x16{};
@@ -381,6 +383,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         product<T>(dps, gf, [&](int, int ks) { return L::row_frag(lv[s], lane & 31, ks, h); });
         const bool part = !u || __any(row.lim < j0 + KT - 1);
         float ds[16];
+        const float d0 = (float)(row.pos - j0 - 4 * h);
         auto grads = [&](auto masked) {
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
@@ -391,7 +394,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
                     float p;
-                    pair_grad<CAP, BIAS>(x[r], dp[r] - delta, lse, slope, (float)(row.pos - j), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
+                    pair_grad<CAP, BIAS>(x[r], dp[r] - delta, lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
                 }
             }
         };
@@ -469,7 +472,7 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
     A.rows_padded = p.rows_padded;
     A.row_lse = a->scratch, A.row_delta = a->scratch + p.rows;
     A.row_lim = (int *)(a->scratch + 2 * p.rows), A.row_doc = (int *)(a->scratch + 3 * p.rows);
-    A.row_pos = (int *)(a->scratch + 4 * p.rows), A.row_slope = a->scratch + 5 * p.rows;
+    A.row_pos = a->scratch + 4 * p.rows, A.row_slope = a->scratch + 5 * p.rows;
     int2 *q_rng = reinterpret_cast<int2 *>(a->scratch + (a->slopes ? 6 : 4) * p.rows), *k_rng = q_rng + (int64_t)a->B * p.nq_tiles;
     const hipStream_t st = (hipStream_t)a->stream;
     return for_dtype(a->dtype, [&](auto tt) {
@@ -483,14 +486,16 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
             if (A.Sk) {
                 AttnK K = A;
                 K.ntile = (A.Sk + 32 * p.kw - 1) / (32 * p.kw), K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
-                const dim3 grid((unsigned)((int64_t)K.ntile * A.B * A.Hkv));
+                K.deal = deal(A.B * A.Hkv, K.ntile);
+                const dim3 grid((unsigned)deal_blocks(K.deal));
                 if (p.kw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 2, CAP, BIAS>), grid, dim3(NT), 0, st, K);
                 else hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, CAP, BIAS>), grid, dim3(NT), 0, st, K);
             }
             if (A.Sq) {
                 AttnK Q = A;
                 Q.ntile = (int)(((int64_t)A.Sq * A.G + BM - 1) / BM), Q.doc_rng = k_rng, Q.ndoc_tiles = p.nk_tiles;
-                hipLaunchKernelGGL((attn_dq_kernel<T, DP, CAP, BIAS>), dim3((unsigned)((int64_t)Q.ntile * A.B * A.Hkv)), dim3(NT), 0, st, Q);
+                Q.deal = deal(A.B * A.Hkv, Q.ntile);
+                hipLaunchKernelGGL((attn_dq_kernel<T, DP, CAP, BIAS>), dim3((unsigned)deal_blocks(Q.deal)), dim3(NT), 0, st, Q);
             }
         };
         auto flags = [&](auto dp) {
