@@ -197,18 +197,19 @@ template <typename T, int DP, int ROWS, int NTH> struct Stage {
     }
 };
 
-// acc[n] += sum over the features of frag_a(n, ks) x b[ks]: the LDS reads of BATCH steps are in flight while the step before multiplies.  Left to
-// itself the compiler reads one operand, waits for it and multiplies, and the LDS latency (some 130 cycles, against 32 of the product)
-// is paid in every step; the scheduling barriers keep the batches apart.
-template <typename T, int NACC, int KS, typename F>
-__device__ __forceinline__ void product(f32x16 (&acc)[NACC], const typename Mma<T>::frag (&b)[KS], F &&frag_a) {
-    constexpr int BATCH = sizeof(T) == 4 ? (KS < 2 ? KS : 2) : (KS < 4 ? KS : 4), STEPS = NACC * KS / BATCH;
-    typename Mma<T>::frag f[2][BATCH];
+// acc[n] += sum over the features of frag_a(n, ks) x frag_b(ks): the LDS reads of BATCH steps are in flight while the step before multiplies.  Left
+// to itself the compiler reads one operand, waits for it and multiplies, and the LDS latency (some 130 cycles, against 32 of the
+// product) is paid in every step; the scheduling barriers keep the batches apart.
+template <typename T, int NACC, int KS, int BATCH, typename FA, typename FB>
+__device__ __forceinline__ void product(f32x16 (&acc)[NACC], FA &&frag_a, FB &&frag_b) {
+    constexpr int STEPS = NACC * KS / BATCH;
+    typename Mma<T>::frag f[2][BATCH], g[2][BATCH];
     auto fetch = [&](auto st) {
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const int u = decltype(st)::value * BATCH + i;
             f[decltype(st)::value & 1][i] = frag_a(u / KS, u % KS);
+            g[decltype(st)::value & 1][i] = frag_b(u % KS);
         }
     };
     fetch(std::integral_constant<int, 0>{});
@@ -218,12 +219,13 @@ __device__ __forceinline__ void product(f32x16 (&acc)[NACC], const typename Mma<
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-            const int u = S * BATCH + i;
-            acc[u / KS] = Mma<T>::mma(f[S & 1][i], b[u % KS], acc[u / KS]);
+            const int n = (S * BATCH + i) / KS;
+            acc[n] = Mma<T>::mma(f[S & 1][i], g[S & 1][i], acc[n]);
         }
         __builtin_amdgcn_sched_barrier(0);
     });
 }
+template <typename T, int KS> constexpr int batch_of() { return sizeof(T) == 4 || KS < 4 ? 2 : 4; }
 
 // zeros over `bytes` (a multiple of 16) of LDS by NTH threads
 template <int NTH> __device__ __forceinline__ void clear_lds(char *p, int bytes, int tid) {

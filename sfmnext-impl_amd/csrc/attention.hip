@@ -118,7 +118,7 @@ template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
 };
 
 template <typename T, int DP, int KT, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_fwd_kernel(AttnK A) {
+__global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128 ? 2 : 3) void attn_fwd_kernel(AttnK A) {
     typedef Tile<T, DP> L;
     typedef typename L::frag frag;
     typedef Stage<T, DP, KT, NT> S;
@@ -209,7 +209,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         f32x16 x[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) x[nb] = f32x16{};
-        product<T>(x, qf, [&](int nb, int ks) { return L::row_frag(lk[s], nb * 32 + (lane & 31), ks, h); });
+        product<T, NB, L::KS, batch_of<T, L::KS>()>(
+            x, [&](int nb, int ks) { return L::row_frag(lk[s], nb * 32 + (lane & 31), ks, h); }, [&](int ks) { return qf[ks]; });
         // the mask, where a row of the wave does not see the whole tile
         const bool part = !u || __any(row.lim < t * KT + KT - 1);
         sm.tile(x, A, lv[s], ld[s], kdoc != nullptr, part, t * KT, row.pos, row.lim, row.qd, slope, lane);
@@ -318,7 +319,8 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
         if (kdoc && lane < 32) ld[wave][lane] = j0 + lane < len ? kdoc[j0 + lane] : -1;
         const char *lk = buf[wave] + s * 2 * S::BYTES, *lv = lk + S::BYTES;
         f32x16 x[1] = {f32x16{}};
-        product<T>(x, qf, [&](int, int ks) { return L::row_frag(lk, lane & 31, ks, h); });
+        product<T, 1, L::KS, batch_of<T, L::KS>()>(
+            x, [&](int, int ks) { return L::row_frag(lk, lane & 31, ks, h); }, [&](int ks) { return qf[ks]; });
         const bool part = kdoc != nullptr || __any(row.lim < j0 + 31);
         sm.tile(x, A, lv, ld[wave], kdoc != nullptr, part, j0, row.pos, row.lim, row.qd, slope, lane);
         t += NW;

@@ -75,17 +75,21 @@ __device__ __forceinline__ void pair_grad(float raw, float e, float lse, float s
     ds = CAP ? q * e * fmaf(-t, t, 1.f) : q * e;
 }
 
-// 4 waves: KW of them side by side on 32 keys each, 4 / KW on the halves of a row tile.
-template <typename T, int DP, int KW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_kernel(AttnK A) {
-    constexpr int QW = 4 / KW, QT = 32 * QW, DB = DP / 32;
+// KW waves side by side on 32 keys each, times QW on the 32-row parts of a row tile.  A wave needs its gK and gV sums (64 registers each at 128
+// features) and the operands of its keys (32 + 32): with those in registers one wave fits a SIMD and every latency is paid.  KVL keeps the keys'
+// operands in LDS instead: 8 waves of 256 registers, two a SIMD.
+template <typename T, int DP, int KW, int QW, bool KVL, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_kernel(AttnK A) {
+    constexpr int NT = 64 * KW * QW, QT = 32 * QW, DB = DP / 32;
     typedef Tile<T, DP> L;
     typedef typename L::frag frag;
     typedef Stage<T, DP, QT, NT> S;
-    __shared__ __align__(16) char lq[2][S::BYTES], lg[2][S::BYTES];
+    typedef Stage<T, DP, 32 * KW, NT> SK;
+    __shared__ __align__(16) char lrow[4][S::BYTES];           // q, q, go, go
+    __shared__ __align__(16) char lk[KVL ? SK::BYTES : 16], lv[KVL ? SK::BYTES : 16];
     __shared__ __align__(16) float rows[2][6 * QT];            // lse, delta, last key, document; with a bias position, slope
-    __shared__ int wk[8];
-    static_assert(QW == 1 || sizeof(lq) >= (size_t)KW * (QW - 1) * 64 * DB * 16 * 4, "a wave's sums fit the row buffers");
+    __shared__ int wk[2 * KW];
+    static_assert(QW == 1 || sizeof(lrow) >= (size_t)KW * (QW - 1) * 64 * DB * 16 * 4, "a wave's sums fit the row buffers");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, kw = wave % KW, qw = wave / KW;
     int bh, tile;                                              // the first keys (the most rows, in causal order) first
@@ -100,8 +104,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
     if (docs && jl < len) kd = A.k_docs[(int64_t)b * A.Sk + jl];
     const bool on = jl < len && (!docs || kd >= 0);
     if (docs && !on) kd = -3;
-    clear_lds<NT>(lq[0], 2 * S::BYTES, tid);
-    clear_lds<NT>(lg[0], 2 * S::BYTES, tid);
+    clear_lds<NT>(lrow[0], 4 * S::BYTES, tid);
 
     int dlo = 0, dhi = 0, wlo = 0, whi = 0;                    // documents of the workgroup's keys, of the wave's
     if (docs) {
@@ -111,12 +114,18 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
             wlo = min(wlo, __shfl_xor(wlo, o, 64));
             whi = max(whi, __shfl_xor(whi, o, 64));
         }
-        if (lane == 0) wk[wave] = wlo, wk[4 + wave] = whi;
+        if (lane == 0 && qw == 0) wk[kw] = wlo, wk[KW + kw] = whi;
+    }
+    if (KVL) {
+        clear_lds<NT>(lk, sizeof(lk), tid);
+        clear_lds<NT>(lv, sizeof(lv), tid);
     }
     __syncthreads();
     if (docs) {
-        dlo = __builtin_amdgcn_readfirstlane(min(min(wk[0], wk[1]), min(wk[2], wk[3])));
-        dhi = __builtin_amdgcn_readfirstlane(max(max(wk[4], wk[5]), max(wk[6], wk[7])));
+        dlo = wk[0], dhi = wk[KW];
+#pragma unroll
+        for (int k = 1; k < KW; ++k) dlo = min(dlo, wk[k]), dhi = max(dhi, wk[KW + k]);
+        dlo = __builtin_amdgcn_readfirstlane(dlo), dhi = __builtin_amdgcn_readfirstlane(dhi);
     }
     const int nt = (RT + QT - 1) / QT;
     // rows that see a key >= j0: all of them, in causal order those from query j0 - off on (a prefix past j0: all)
@@ -127,13 +136,29 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
     const bool all_on = __all(on);
     const float jf = (float)jl;
 
-    frag kf[L::KS], vf[L::KS];
-    const T *krow = (const T *)A.k + b * A.ks[0] + (int64_t)jl * A.ks[1] + hk * A.ks[2];
-    const T *vrow = (const T *)A.v + b * A.vs[0] + (int64_t)jl * A.vs[1] + hk * A.vs[2];
+    frag kf[KVL ? 1 : L::KS], vf[KVL ? 1 : L::KS];
+    const T *kbase = (const T *)A.k + b * A.ks[0] + (int64_t)j0 * A.ks[1] + hk * A.ks[2];
+    const T *vbase = (const T *)A.v + b * A.vs[0] + (int64_t)j0 * A.vs[1] + hk * A.vs[2];
+    if constexpr (KVL) {                                       // padding keys hold anything and are not loaded
+        SK sk, sv;
+        sk.aim(tid, (unsigned)A.ks[1]);
+        sv.aim(tid, (unsigned)A.vs[1]);
+        int kp[SK::N];
+        if (docs)
 #pragma unroll
-    for (int ks = 0; ks < L::KS; ++ks) {
-        kf[ks] = L::mem_frag(krow, ks, h, A.D, on);
-        vf[ks] = L::mem_frag(vrow, ks, h, A.D, on);
+            for (int n = 0; n < SK::N; ++n) {
+                const int r = SK::piece_row(n, tid, A.D);
+                kp[n] = r < len - j0 ? A.k_docs[(int64_t)b * A.Sk + j0 + r] : -1;
+            }
+        sk.load(kbase, lds_offset(lk), tid, A.D, len - j0, docs, kp);
+        sv.load(vbase, lds_offset(lv), tid, A.D, len - j0, docs, kp);
+    } else {
+        const T *krow = kbase + (int64_t)(jl - j0) * A.ks[1], *vrow = vbase + (int64_t)(jl - j0) * A.vs[1];
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ++ks) {
+            kf[ks] = L::mem_frag(krow, ks, h, A.D, on);
+            vf[ks] = L::mem_frag(vrow, ks, h, A.D, on);
+        }
     }
 
     const T *qb = (const T *)A.q + b * A.qs[0] + (int64_t)hk * A.G * A.qs[2], *gb = (const T *)A.go + b * A.gos[0] + (int64_t)hk * A.G * A.gos[2];
@@ -141,7 +166,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
     S sq, sg;
     sq.aim_packed(tid, 0, A.G, A.g_magic, (unsigned)A.qs[1], (unsigned)A.qs[2]);
     sg.aim_packed(tid, 0, A.G, A.g_magic, (unsigned)A.gos[1], (unsigned)A.gos[2]);
-    const unsigned oq = lds_offset(lq[0]), og = lds_offset(lg[0]), orow = lds_offset(rows[0]);
+    const unsigned oq = lds_offset(lrow[0]), og = oq + 2 * S::BYTES, orow = lds_offset(rows[0]);
     // rows that see no key hold anything and are not loaded: their limits are read a tile ahead of the DMA that goes by them
     const bool skips = docs || (A.causal && off < 0 && prefix <= 0);
     int pd[S::N];
@@ -188,6 +213,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
         peek(t2);
         const int q0 = qw * 32;
         const float *rw = rows[s];
+        const char *lq = lrow[s], *lg = lrow[2 + s];
         f32x16 xs[1] = {f32x16{}}, dps[1];                     // dP starts from -delta
         f32x16 &x = xs[0], &dp = dps[0];
 #pragma unroll
@@ -196,8 +222,11 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
 #pragma unroll
             for (int e = 0; e < 4; ++e) dp[4 * r4 + e] = -d[e];
         }
-        product<T>(xs, kf, [&](int, int ks) { return L::row_frag(lq[s], q0 + (lane & 31), ks, h); });
-        product<T>(dps, vf, [&](int, int ks) { return L::row_frag(lg[s], q0 + (lane & 31), ks, h); });
+        constexpr int BATCH = KVL ? 2 : batch_of<T, L::KS>();
+        product<T, 1, L::KS, BATCH>(xs, [&](int, int ks) { return L::row_frag(lq, q0 + (lane & 31), ks, h); },
+                                    [&](int ks) { return KVL ? L::row_frag(lk, kw * 32 + (lane & 31), ks, h) : kf[KVL ? 0 : ks]; });
+        product<T, 1, L::KS, BATCH>(dps, [&](int, int ks) { return L::row_frag(lg, q0 + (lane & 31), ks, h); },
+                                    [&](int ks) { return KVL ? L::row_frag(lv, kw * 32 + (lane & 31), ks, h) : vf[KVL ? 0 : ks]; });
         // every row of the tile sees all of the wave's keys?  (limits do not fall with the row)
         const int R0 = t * QT + q0;
         const bool part = !all_on || !u || R0 + 32 > RT || row_limit(div_g(R0, A.g_magic) + off, len, A.causal, prefix) < j0 + kw * 32 + 31;
@@ -225,13 +254,13 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
         // gV, gK for 16 rows, then for the other 16; the operands of a step are read while the step before multiplies
         frag cf[2][DB];
 #pragma unroll
-        for (int db = 0; db < DB; ++db) cf[0][db] = L::col_frag(lg[s], q0, db, lane);
+        for (int db = 0; db < DB; ++db) cf[0][db] = L::col_frag(lg, q0, db, lane);
         static_for<4>([&](auto step) {
             constexpr int K = decltype(step)::value;
             const frag f = Mma<T>::pack((K & 1 ? ds : p) + 8 * (K / 2));
             if constexpr (K < 3)
 #pragma unroll
-                for (int db = 0; db < DB; ++db) cf[(K + 1) & 1][db] = L::col_frag(K & 1 ? lg[s] : lq[s], q0 + (K + 1) / 2 * 16, db, lane);
+                for (int db = 0; db < DB; ++db) cf[(K + 1) & 1][db] = L::col_frag(K & 1 ? lg : lq, q0 + (K + 1) / 2 * 16, db, lane);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
@@ -246,7 +275,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_ke
         t = tn, u = un, tn = t2, un = u2;
     }
     if (QW > 1) {                                              // the row halves' sums, through the row buffers: gK, then gV
-        float *red = reinterpret_cast<float *>(lq[0]);
+        float *red = reinterpret_cast<float *>(lrow[0]);
         auto join = [&](f32x16 (&g)[DB]) {
             if (qw > 0)
 #pragma unroll
@@ -379,8 +408,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         const int j0 = t * KT;
         f32x16 xs[1] = {f32x16{}}, dps[1] = {f32x16{}};
         f32x16 &x = xs[0], &dp = dps[0];
-        product<T>(xs, qf, [&](int, int ks) { return L::row_frag(lk[s], lane & 31, ks, h); });
-        product<T>(dps, gf, [&](int, int ks) { return L::row_frag(lv[s], lane & 31, ks, h); });
+        product<T, 1, L::KS, batch_of<T, L::KS>()>(xs, [&](int, int ks) { return L::row_frag(lk[s], lane & 31, ks, h); }, [&](int ks) { return qf[ks]; });
+        product<T, 1, L::KS, batch_of<T, L::KS>()>(dps, [&](int, int ks) { return L::row_frag(lv[s], lane & 31, ks, h); }, [&](int ks) { return gf[ks]; });
         const bool part = !u || __any(row.lim < j0 + KT - 1);
         float ds[16];
         const float d0 = (float)(row.pos - j0 - 4 * h);
@@ -429,13 +458,17 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         }
 }
 
-struct BwdPlan { int kw, rows_padded, nq_tiles, nk_tiles; int64_t rows, scratch; };
+struct BwdPlan { int kw, qw, rows_padded, nq_tiles, nk_tiles; int64_t rows, scratch; };
 BwdPlan bwd_plan(const sqd_attn_args *a) {
     BwdPlan p{};
     const int G = a->Hq / a->Hkv;
-    // keys a workgroup: 128, or 64 with the row tile split between the waves while 128 would leave CUs idle or a last round nearly empty
-    p.kw = (int64_t)((a->Sk + 127) / 128) * a->B * a->Hkv < 1024 ? 2 : 4;
-    const int QT = 32 * (4 / p.kw);
+    // keys and row parts of a workgroup: 128 x 2 with 8 waves where that fits (16-bit types past 64 features) and gives most CUs a workgroup; else 4
+    // waves, 64 x 2 while 128 x 1 would leave CUs idle or a last round nearly empty
+    const int64_t wide = (int64_t)((a->Sk + 127) / 128) * a->B * a->Hkv;
+    if (a->dtype != SQD_F32 && a->D > 64 && wide >= 192) p.kw = 4, p.qw = 2;
+    else if (wide < 1024) p.kw = 2, p.qw = 2;
+    else p.kw = 4, p.qw = 1;
+    const int QT = 32 * p.qw;
     p.rows_padded = (a->Sq * G + 63) / 64 * 64;
     p.rows = (int64_t)a->B * a->Hkv * p.rows_padded;
     p.nq_tiles = a->q_docs ? (a->Sq * G + QT - 1) / QT : 0;
@@ -478,7 +511,7 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);
         if (p.rows) hipLaunchKernelGGL((attn_rows_kernel<T>), dim3(p.rows_padded / 16, A.Hkv, A.B), dim3(NT), 0, st, A);
-        if (p.nq_tiles) attn_doc_ranges(A.q_docs, q_rng, A.B, A.Sq, A.G, 32 * (4 / p.kw), p.nq_tiles, st);
+        if (p.nq_tiles) attn_doc_ranges(A.q_docs, q_rng, A.B, A.Sq, A.G, 32 * p.qw, p.nq_tiles, st);
         if (p.nk_tiles) attn_doc_ranges(A.k_docs, k_rng, A.B, A.Sk, 1, 32, p.nk_tiles, st);
         auto go = [&](auto dp, auto cap, auto bias) {
             constexpr int DP = decltype(dp)::value;
@@ -488,8 +521,11 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
                 K.ntile = (A.Sk + 32 * p.kw - 1) / (32 * p.kw), K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
                 K.deal = deal(A.B * A.Hkv, K.ntile);
                 const dim3 grid((unsigned)deal_blocks(K.deal));
-                if (p.kw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 2, CAP, BIAS>), grid, dim3(NT), 0, st, K);
-                else hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, CAP, BIAS>), grid, dim3(NT), 0, st, K);
+                if constexpr (sizeof(T) == 2 && DP == 128) {
+                    if (p.kw == 4 && p.qw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 2, true, CAP, BIAS>), grid, dim3(512), 0, st, K);
+                }
+                if (p.kw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 2, 2, false, CAP, BIAS>), grid, dim3(NT), 0, st, K);
+                else if (p.qw == 1) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 1, false, CAP, BIAS>), grid, dim3(NT), 0, st, K);
             }
             if (A.Sq) {
                 AttnK Q = A;
