@@ -36,6 +36,7 @@ struct AttnK {
     unsigned g_magic;
     Deal deal;
     float unit_inv;                          // slopes are used in units of the raw score (1 / scale) or of tanh (1 / cap)
+    float *part_a, *part_b;                  // the backward's parts where the looped-over side is split: [nsplit][gradient's shape]
     int B, Sq, Sk, Hq, Hkv, G, D, causal, ntile, nsplit, ndoc_tiles, rows_padded;
 };
 

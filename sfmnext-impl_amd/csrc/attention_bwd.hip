@@ -92,9 +92,9 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 
     static_assert(QW == 1 || sizeof(lrow) >= (size_t)KW * (QW - 1) * 64 * DB * 16 * 4, "a wave's sums fit the row buffers");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, kw = wave % KW, qw = wave / KW;
-    int bh, tile;                                              // the first keys (the most rows, in causal order) first
-    if (!dealt(A.deal, blockIdx.x, A.ntile, bh, tile)) return;
-    const int hk = bh % A.Hkv, b = bh / A.Hkv;
+    int bh, u0;                                                // the first keys (the most rows, in causal order) first
+    if (!dealt(A.deal, blockIdx.x, A.ntile * A.nsplit, bh, u0)) return;
+    const int tile = u0 / A.nsplit, split = u0 - tile * A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, j0 = tile * 32 * KW, jl = j0 + kw * 32 + (lane & 31);
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk, off = len - A.Sq;
     const int prefix = A.prefix ? A.prefix[b] : 0;
@@ -127,11 +127,16 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 
         for (int k = 1; k < KW; ++k) dlo = min(dlo, wk[k]), dhi = max(dhi, wk[KW + k]);
         dlo = __builtin_amdgcn_readfirstlane(dlo), dhi = __builtin_amdgcn_readfirstlane(dhi);
     }
-    const int nt = (RT + QT - 1) / QT;
+    int nt = (RT + QT - 1) / QT;
     // rows that see a key >= j0: all of them, in causal order those from query j0 - off on (a prefix past j0: all)
     int t0 = 0;
     if (A.causal && prefix <= j0) t0 = (int)(min((int64_t)max(j0 - off, 0) * A.G, (int64_t)RT) / QT);
     if (j0 >= len) t0 = nt;
+    if (A.nsplit > 1) {
+        const int per = (nt - t0 + A.nsplit - 1) / A.nsplit;
+        t0 = min(nt, t0 + split * per);
+        nt = min(nt, t0 + per);
+    }
     DocWalk walk(docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, nt);
     const bool all_on = __all(on);
     const float jf = (float)jl;
@@ -306,6 +311,12 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 
             if (d >= A.D) continue;
             const float a[4] = {gk[db][4 * r4] * A.scale, gk[db][4 * r4 + 1] * A.scale, gk[db][4 * r4 + 2] * A.scale, gk[db][4 * r4 + 3] * A.scale};
             const float c[4] = {gv[db][4 * r4], gv[db][4 * r4 + 1], gv[db][4 * r4 + 2], gv[db][4 * r4 + 3]};
+            if (A.nsplit > 1) {
+                const int64_t at = (int64_t)split * A.B * A.Sk * A.Hkv * A.D + o + d;
+                store_f32<float, 4>(A.part_a + at, a);
+                store_f32<float, 4>(A.part_b + at, c);
+                continue;
+            }
             store_f32<T, 4>((T *)A.gk + o + d, a);
             store_f32<T, 4>((T *)A.gv + o + d, c);
         }
@@ -323,8 +334,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     int bh, w;
-    if (!dealt(A.deal, blockIdx.x, A.ntile, bh, w)) return;
-    const int tile = A.ntile - 1 - w, hk = bh % A.Hkv, b = bh / A.Hkv;
+    if (!dealt(A.deal, blockIdx.x, A.ntile * A.nsplit, bh, w)) return;
+    const int split = w % A.nsplit, tile = A.ntile - 1 - w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, row0 = tile * BM;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
     const int prefix = A.prefix ? A.prefix[b] : 0;
@@ -349,7 +360,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         dlo = __builtin_amdgcn_readfirstlane(min(min(wq[0], wq[1]), min(wq[2], wq[3])));
         dhi = __builtin_amdgcn_readfirstlane(max(max(wq[4], wq[5]), max(wq[6], wq[7])));
     }
-    const int t1 = (kend + KT - 1) / KT;
+    const int nt_all = (kend + KT - 1) / KT, per = (nt_all + A.nsplit - 1) / A.nsplit, t0 = min(nt_all, split * per), t1 = min(nt_all, t0 + per);
     DocWalk walk(A.q_docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, t1);
 
     frag qf[L::KS], gf[L::KS];
@@ -393,7 +404,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
 
     int s = 0;
     bool u, un;
-    int t = walk.next(0, u);
+    int t = walk.next(t0, u);
     peek(t);
     if (t < t1) fetch(t, 0);
     int tn = walk.next(t + 1, un);
@@ -447,18 +458,43 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         t = tn, u = un, tn = t2, un = u2;
     }
     if (!row.on) return;
-    T *out = (T *)A.gq + (((int64_t)b * A.Sq + row.i) * A.Hq + hk * A.G + row.g) * A.D;
+    const int64_t out = (((int64_t)b * A.Sq + row.i) * A.Hq + hk * A.G + row.g) * A.D;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
             const int d = db * 32 + 8 * r4 + 4 * h;
             const float v[4] = {gq[db][4 * r4] * A.scale, gq[db][4 * r4 + 1] * A.scale, gq[db][4 * r4 + 2] * A.scale, gq[db][4 * r4 + 3] * A.scale};
-            if (d < A.D) store_f32<T, 4>(out + d, v);
+            if (d >= A.D) continue;
+            if (A.nsplit > 1) store_f32<float, 4>(A.part_a + (int64_t)split * A.B * A.Sq * A.Hq * A.D + out + d, v);
+            else store_f32<T, 4>((T *)A.gq + out + d, v);
         }
 }
 
-struct BwdPlan { int kw, qw, rows_padded, nq_tiles, nk_tiles; int64_t rows, scratch; };
+// out = the parts of a gradient, added in order
+template <typename T>
+__global__ __launch_bounds__(NT) void attn_parts_kernel(const float *__restrict__ part, T *__restrict__ out, int64_t n4, int nsplit) {
+    const int64_t u = (int64_t)blockIdx.x * NT + threadIdx.x;
+    if (u >= n4) return;
+    float a[4];
+    load_f32<float, 4>(part + u * 4, a);
+    for (int s = 1; s < nsplit; ++s) {
+        float b[4];
+        load_f32<float, 4>(part + (s * n4 + u) * 4, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] += b[e];
+    }
+    store_f32<T, 4>(out + u * 4, a);
+}
+
+struct BwdPlan { int kw, qw, rows_padded, nq_tiles, nk_tiles, k_split, q_split; int64_t rows, nk, nq, parts, scratch; };
+// parts of the looped-over side: with fewer than 192 workgroups CUs idle, and 512 shorter ones also even out causal rows (168 of fp32, 1281 tokens:
+// dK dV 214 -> 108 us in 3 parts); at least 8 tiles each.  With 240 (3 documents, 3840 tokens) parts lose: 306 -> 493 us, documents being uneven in them.
+int parts_of(int64_t blocks, int64_t tiles) {
+    int64_t n = blocks && blocks < 192 ? 512 / blocks : 1;
+    n = n > tiles / 8 ? tiles / 8 : n;
+    return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+}
 BwdPlan bwd_plan(const sqd_attn_args *a) {
     BwdPlan p{};
     const int G = a->Hq / a->Hkv;
@@ -473,7 +509,12 @@ BwdPlan bwd_plan(const sqd_attn_args *a) {
     p.rows = (int64_t)a->B * a->Hkv * p.rows_padded;
     p.nq_tiles = a->q_docs ? (a->Sq * G + QT - 1) / QT : 0;
     p.nk_tiles = a->q_docs ? (a->Sk + 31) / 32 : 0;
-    p.scratch = (a->slopes ? 6 : 4) * p.rows + (int64_t)2 * a->B * (p.nq_tiles + p.nk_tiles);
+    p.nk = (int64_t)a->B * a->Sk * a->Hkv * a->D, p.nq = (int64_t)a->B * a->Sq * a->Hq * a->D;
+    p.k_split = parts_of((int64_t)((a->Sk + 32 * p.kw - 1) / (32 * p.kw)) * a->B * a->Hkv, (a->Sq * G + QT - 1) / QT);
+    p.q_split = parts_of((int64_t)((a->Sq * G + BM - 1) / BM) * a->B * a->Hkv, (a->Sk + 31) / 32);
+    const int64_t pk = p.k_split > 1 ? 2 * p.k_split * p.nk : 0, pq = p.q_split > 1 ? p.q_split * p.nq : 0;      // one after the other
+    p.parts = (a->slopes ? 6 : 4) * p.rows + ((int64_t)2 * a->B * (p.nq_tiles + p.nk_tiles) + 3) / 4 * 4;
+    p.scratch = p.parts + (pk > pq ? pk : pq);
     return p;
 }
 }  // namespace
@@ -519,19 +560,28 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
             if (A.Sk) {
                 AttnK K = A;
                 K.ntile = (A.Sk + 32 * p.kw - 1) / (32 * p.kw), K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
-                K.deal = deal(A.B * A.Hkv, K.ntile);
+                K.nsplit = p.k_split, K.part_a = a->scratch + p.parts, K.part_b = K.part_a + p.k_split * p.nk;
+                K.deal = deal(A.B * A.Hkv, K.ntile * K.nsplit);
                 const dim3 grid((unsigned)deal_blocks(K.deal));
                 if constexpr (sizeof(T) == 2 && DP == 128) {
                     if (p.kw == 4 && p.qw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 2, true, CAP, BIAS>), grid, dim3(512), 0, st, K);
                 }
                 if (p.kw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 2, 2, false, CAP, BIAS>), grid, dim3(NT), 0, st, K);
                 else if (p.qw == 1) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 1, false, CAP, BIAS>), grid, dim3(NT), 0, st, K);
+                if (K.nsplit > 1) {                                // (parts of dK, dV are joined before the scratch holds dQ's)
+                    const dim3 g2((unsigned)((p.nk / 4 + NT - 1) / NT));
+                    hipLaunchKernelGGL((attn_parts_kernel<T>), g2, dim3(NT), 0, st, K.part_a, (T *)a->gk, p.nk / 4, K.nsplit);
+                    hipLaunchKernelGGL((attn_parts_kernel<T>), g2, dim3(NT), 0, st, K.part_b, (T *)a->gv, p.nk / 4, K.nsplit);
+                }
             }
             if (A.Sq) {
                 AttnK Q = A;
                 Q.ntile = (int)(((int64_t)A.Sq * A.G + BM - 1) / BM), Q.doc_rng = k_rng, Q.ndoc_tiles = p.nk_tiles;
-                Q.deal = deal(A.B * A.Hkv, Q.ntile);
+                Q.nsplit = p.q_split, Q.part_a = a->scratch + p.parts;
+                Q.deal = deal(A.B * A.Hkv, Q.ntile * Q.nsplit);
                 hipLaunchKernelGGL((attn_dq_kernel<T, DP, CAP, BIAS>), dim3((unsigned)deal_blocks(Q.deal)), dim3(NT), 0, st, Q);
+                if (Q.nsplit > 1)
+                    hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)((p.nq / 4 + NT - 1) / NT)), dim3(NT), 0, st, Q.part_a, (T *)a->gq, p.nq / 4, Q.nsplit);
             }
         };
         auto flags = [&](auto dp) {

@@ -336,9 +336,23 @@ def bins_head(energy_maps, conv1x1, y, min_val, max_val, raw_linear=False):
 
 
 # ---- token operators of image / video encoders (csrc/token_norm.hip, rotary.hip, attention*.hip) --------------------------------------
+_tokens = None
+
+
+def _token_kernels():
+    global _tokens
+    if _tokens is None:                # bound at the first call: importing this module needs no built library
+        from . import tokens
+        _tokens = tokens
+    return _tokens
+
+
 def _token_tensor(who, name, t, dim, like=None):
     """the checks that every tensor of a token operator passes; `like`: same element type and device"""
-    from . import tokens
+    tokens = _token_kernels()
+    if isinstance(t, torch.Tensor) and t.dim() == dim and t.is_cuda and t.dtype in tokens.DTYPE and (
+            like is None or (t.dtype == like.dtype and t.device == like.device)):
+        return
     if not isinstance(t, torch.Tensor) or t.dim() != dim:
         raise RuntimeError("sqd: %s: %s must be a tensor of %d dimensions" % (who, name, dim))
     if not t.is_cuda:
@@ -373,7 +387,7 @@ def rms_norm_residual(x, weight, residual=None, eps=1e-6):
             raise RuntimeError("sqd: %s: residual %s against x %s" % (who, tuple(residual.shape), tuple(x.shape)))
     if not eps >= 0.0:
         raise RuntimeError("sqd: %s: eps = %r" % (who, eps))
-    from . import tokens
+    tokens = _token_kernels()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         out = tokens.RmsNormResidual.apply(x, weight, residual, float(eps))
         return out if residual is not None else (out, x)
@@ -413,7 +427,7 @@ def rotary_axes(q, k, positions, freq, pairs, interleaved=False):
         raise RuntimeError("sqd: %s: positions must be [S,A] or [B,S,A]" % who)
     positions = _index_tensor(who, "positions", positions, ((S,) if positions.dim() == 2 else (B, S)) + (len(pairs),), q.device, (torch.int32, torch.int64))
     freq = _index_tensor(who, "freq", freq, (P,), q.device, (torch.float64,))
-    from . import tokens
+    tokens = _token_kernels()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = tokens.RotaryAxes.apply(q, k, positions, freq, pairs, int(bool(interleaved)))
         return out if k is not None else (out, None)
@@ -462,7 +476,7 @@ def attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefi
         k_docs = _index_tensor(who, "k_docs", k_docs, (B, Sk), q.device, i32)
     if k_len is not None:
         k_len = _index_tensor(who, "k_len", k_len, (B,), q.device, i32)
-    from . import tokens
+    tokens = _token_kernels()
     cfg, masks = (scale, softcap, int(bool(causal))), (slopes, prefix, q_docs, k_docs, k_len)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return tokens.Attention.apply(q, k, v, cfg, *masks)

@@ -172,6 +172,31 @@ def test_attention(n, dtype):
         assert torch.equal(_ops().attention(*d, **_cuda(kw)), o)
 
 
+# the variants a size selects: 128-key workgroups of 8 and of 4 waves, keys or rows split over workgroups (few heads, long sequences), key heads that
+# share an XCD unevenly
+WIDE = [
+    (_case(8, 200, 200, 16, 16, 128, docs=(3, 17), softcap=20.0), BF16), (_case(8, 150, 290, 8, 8, 96, causal=True, k_len=[290, 2, 150, 149, 77, 200, 13, 290]), F16),
+    (_case(6, 129, 129, 70, 70, 16, causal=True, prefix=[0, 1, 50, 129, 200, 128]), BF16), (_case(6, 140, 140, 65, 65, 8, slopes=True), F32),
+    (_case(1, 1100, 1100, 1, 1, 64, causal=True), BF16), (_case(1, 901, 1203, 3, 1, 40, softcap=9.0, causal=True, prefix=[300]), F32),
+    (_case(3, 700, 700, 2, 1, 128, docs=(4, 90), slopes=True), F16), (_case(1, 700, 701, 5, 5, 64, causal=True, k_len=[640]), BF16),
+]
+
+
+@pytest.mark.parametrize("n", range(len(WIDE)))
+def test_attention_variants(n):
+    c, dtype = WIDE[n]
+    q, k, v, go, kw = _build(c, dtype)
+    ref = attention_ref(q, k, v, go=go, **kw)
+    d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    o = _ops().attention(*d, **_cuda(kw))
+    check(o, ref["o"], ref["o_tol"], "o")
+    first = torch.autograd.grad(o, d, go.cuda(), retain_graph=True)
+    for name, got in zip(("gq", "gk", "gv"), first):
+        check(got, ref[name], ref[name + "_tol"], name)
+    for a, b in zip(first, torch.autograd.grad(o, d, go.cuda())):
+        assert torch.equal(a, b)
+
+
 def test_attention_one_key_has_no_score_gradient():
     q, k, v, go, kw = _build(_case(3, 1, 1, 4, 2, 128, causal=True), BF16)
     d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
