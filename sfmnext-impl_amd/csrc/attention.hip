@@ -192,7 +192,6 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
 
     const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * A.unit_inv : 0.f;
     Softmax<T, DP, NB, CAP, BIAS> sm;
-    int s = 0;
     bool u, un;
     int t = walk.next(t0, u);
     peek(t);
@@ -201,7 +200,9 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
     peek(tn);
     dma_wait();
     __syncthreads();
-    while (t < t1) {
+    // the two buffers as two copies of the loop body: LDS addresses are then constants of a lane (40 of 295 vector instructions a tile less)
+    auto step = [&](auto buffer) __attribute__((always_inline)) {
+        constexpr int s = decltype(buffer)::value;
         if (tn < t1) fetch(tn, s ^ 1);
         bool u2 = true;
         const int t2 = walk.next(tn + 1, u2);
@@ -216,8 +217,12 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
         sm.tile(x, A, lv[s], ld[s], kdoc != nullptr, part, t * KT, row.pos, row.lim, row.qd, slope, lane);
         dma_wait();
         __syncthreads();
-        s ^= 1;
         t = tn, u = un, tn = t2, un = u2;
+    };
+    while (t < t1) {
+        step(std::integral_constant<int, 0>{});
+        if (t >= t1) break;
+        step(std::integral_constant<int, 1>{});
     }
 
     const float l = half_sum(sm.l), inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -264,9 +269,8 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
     __shared__ float wm[NW][32], wl[NW][32];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    int bh, split;
-    if (!dealt(A.deal, blockIdx.x, A.nsplit, bh, split)) return;
-    const int hk = bh % A.Hkv, b = bh / A.Hkv;
+    // no two workgroups share keys: the splits of a row of the batch, whose lengths differ, go round the XCDs
+    const int groups = A.B * A.Hkv, split = blockIdx.x / groups, bh = blockIdx.x - split * groups, hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, R = lane & 31;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
     const int prefix = A.prefix ? A.prefix[b] : 0;
@@ -411,9 +415,11 @@ Split plan(const sqd_attn_args *a) {
     p.token = rows <= 32;
     const int KT = p.token ? 32 : a->dtype == SQD_F32 ? 32 : 64;
     const int64_t groups = (int64_t)a->B * a->Hkv * (p.token ? 1 : (rows + BM - 1) / BM);
-    // two workgroups fit a CU: split the keys while fewer than 512 would run, down to 256 keys for each
+    // split the keys while CUs would idle, down to 256 keys for each: two workgroups of the row kernel fit a CU; of the token kernel as many as its
+    // buffers leave room for (one at 128 features of 16 bits: 512 instead of 256 workgroups cost 95 against 87 us on 16 x 8 key heads of 8191)
+    const int bytes = pad_dim(a->D) * (a->dtype == SQD_F32 ? 4 : 2), want = p.token ? 256 * (bytes >= 256 ? 1 : 256 / bytes) : 512;
     const int tiles = (a->Sk + KT - 1) / KT;
-    int64_t n = groups ? 512 / groups : 1;
+    int64_t n = groups ? want / groups : 1;
     n = n > a->Sk / 256 ? a->Sk / 256 : n;
     p.nsplit = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     p.ndoc_tiles = a->q_docs && !p.token ? tiles : 0;
@@ -491,7 +497,7 @@ extern "C" int sqd_attn_fwd(const sqd_attn_args *a) {
     const int64_t tiles = (int64_t)A.ntile * A.nsplit;
     SQD_CHECK_ARG(tiles < (1 << 24), "sqd_attn_fwd: too many tokens");
     A.deal = deal(A.B * A.Hkv, (int)tiles);
-    const int64_t blocks = deal_blocks(A.deal);
+    const int64_t blocks = p.token ? tiles * A.B * A.Hkv : deal_blocks(A.deal);
     SQD_CHECK_ARG(blocks < (1ll << 31), "sqd_attn_fwd: too many tokens");
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);
