@@ -398,9 +398,11 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         if (kdoc && tid < KT) ld[s][tid] = sd;
     };
     const float slope = BIAS && row.on ? A.slopes[hk * A.G + row.g] * A.unit_inv : 0.f;
-    f32x16 gq[DB];
+    f32x16 gq[DB], minus_delta;                                // dP starts from -delta: 16 registers against 16 subtractions a step
 #pragma unroll
     for (int db = 0; db < DB; ++db) gq[db] = f32x16{};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
 
     int s = 0;
     bool u, un;
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         const int t2 = walk.next(tn + 1, u2);
         peek(t2);
         const int j0 = t * KT;
-        f32x16 xs[1] = {f32x16{}}, dps[1] = {f32x16{}};
+        f32x16 xs[1] = {f32x16{}}, dps[1] = {minus_delta};
         f32x16 &x = xs[0], &dp = dps[0];
         product<T, 1, L::KS, batch_of<T, L::KS>()>(xs, [&](int, int ks) { return L::row_frag(lk[s], lane & 31, ks, h); }, [&](int ks) { return qf[ks]; });
         product<T, 1, L::KS, batch_of<T, L::KS>()>(dps, [&](int, int ks) { return L::row_frag(lv[s], lane & 31, ks, h); }, [&](int ks) { return gf[ks]; });
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
                     float p;
-                    pair_grad<CAP, BIAS>(x[r], dp[r] - delta, lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
+                    pair_grad<CAP, BIAS>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
                 }
             }
         };

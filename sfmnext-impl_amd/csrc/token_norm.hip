@@ -198,15 +198,21 @@ __global__ __launch_bounds__(NT) void norm_gw_any_kernel(const T *__restrict__ g
     if (grp == 0 && c < C) part[(int64_t)blockIdx.y * C + c] = red[0][col] + red[1][col] + red[2][col] + red[3][col];
 }
 
-// g_w[c] = sum of the partial rows, in a fixed order: 16 columns x 16 row groups, then a tree over the groups
+// g_w[c] = sum of the partial rows, in a fixed order: 16 columns x 16 row groups, eight loads of a group under way at a time, then a tree over the
+// groups
 template <typename W>
 __global__ __launch_bounds__(NT) void norm_gw_reduce_kernel(const float *__restrict__ part, W *__restrict__ gw, int nparts, int C) {
     __shared__ float red[16][17];
     const int col = threadIdx.x & 15, grp = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
-    float a = 0.f;
-    if (c < C)
-        for (int p = grp; p < nparts; p += 16) a += part[(int64_t)p * C + c];
-    red[grp][col] = a;
+    float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < C) {
+        int p = grp;
+        for (; p + 16 * 7 < nparts; p += 16 * 8)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) a[k] += part[(int64_t)(p + 16 * k) * C + c];
+        for (; p < nparts; p += 16) a[0] += part[(int64_t)p * C + c];
+    }
+    red[grp][col] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
     __syncthreads();
 #pragma unroll
     for (int k = 8; k > 0; k >>= 1) {
