@@ -211,11 +211,20 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 
     peek(tn);
     dma_wait();
     __syncthreads();
+    // Two waves of a SIMD that meet at one barrier a tile do their products at the same time and their exponentials at the same time.  With
+    // 8 waves the second four run half a tile behind: two barriers a tile, the first four pass [products, half of the pairs] while the others pass
+    // [half of the pairs, products].  A tile's buffer is then free half a tile later, so the first four fetch in mid-tile; the loads of either
+    // have the half tile up to the same barrier.
+    constexpr bool STAGGER = KW * QW == 8;
+    const bool late = STAGGER && qw == 1;
+    auto meet = [] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if (late) meet();
     while (t < nt) {
-        if (tn < nt) fetch(tn, s ^ 1);
-        bool u2 = true;
-        const int t2 = walk.next(tn + 1, u2);
-        peek(t2);
+        if ((!STAGGER || late) && tn < nt) fetch(tn, s ^ 1);
         const int q0 = qw * 32;
         const float *rw = rows[s];
         const char *lq = lrow[s], *lg = lrow[2 + s];
@@ -235,11 +244,14 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 
         // every row of the tile sees all of the wave's keys?  (limits do not fall with the row)
         const int R0 = t * QT + q0;
         const bool part = !all_on || !u || R0 + 32 > RT || row_limit(div_g(R0, A.g_magic) + off, len, A.causal, prefix) < j0 + kw * 32 + 31;
-        float p[16], ds[16];
-        auto grads = [&](auto masked) {
+        // 8 registers (16 rows of the tile) at a time: probabilities and score gradients, then their shares of gV and gK.  The second half's pairs
+        // run under the first half's products.
+        float p[8], ds[8];
+        auto pairs = [&](auto half, auto masked) {
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int q4 = q0 + 8 * r4 + 4 * h;
+            for (int r2 = 0; r2 < 2; ++r2) {
+                constexpr int H = decltype(half)::value;
+                const int q4 = q0 + 8 * (2 * H + r2) + 4 * h;
                 const f32x4 lse = *reinterpret_cast<const f32x4 *>(rw + q4);
                 int4 lim = make_int4(0, 0, 0, 0), qd = make_int4(kd, kd, kd, kd);
                 f32x4 ps = {0, 0, 0, 0}, sl = {0, 0, 0, 0};
@@ -248,37 +260,59 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 
                 if (BIAS) ps = *reinterpret_cast<const f32x4 *>(rw + 4 * QT + q4), sl = *reinterpret_cast<const f32x4 *>(rw + 5 * QT + q4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = r4 * 4 + e;
+                    const int r = (2 * H + r2) * 4 + e;
                     const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
-                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), p[r], ds[r]);
+                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), p[r2 * 4 + e], ds[r2 * 4 + e]);
                 }
             }
         };
-        if (part) grads(std::true_type{});
-        else grads(std::false_type{});
-        // gV, gK for 16 rows, then for the other 16; the operands of a step are read while the step before multiplies
-        frag cf[2][DB];
+        auto grads = [&](auto half) {
+            if (part) pairs(half, std::true_type{});
+            else pairs(half, std::false_type{});
+        };
+        frag cg[DB], cq[DB], pf, df;
+        auto operands = [&](int row) {
 #pragma unroll
-        for (int db = 0; db < DB; ++db) cf[0][db] = L::col_frag(lg, q0, db, lane);
-        static_for<4>([&](auto step) {
-            constexpr int K = decltype(step)::value;
-            const frag f = Mma<T>::pack((K & 1 ? ds : p) + 8 * (K / 2));
-            if constexpr (K < 3)
+            for (int db = 0; db < DB; ++db) cg[db] = L::col_frag(lg, q0 + row, db, lane);
 #pragma unroll
-                for (int db = 0; db < DB; ++db) cf[(K + 1) & 1][db] = L::col_frag(K & 1 ? lg : lq, q0 + (K + 1) / 2 * 16, db, lane);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int db = 0; db < DB; ++db) cq[db] = L::col_frag(lq, q0 + row, db, lane);
+        };
+        auto products = [&] {
 #pragma unroll
-            for (int db = 0; db < DB; ++db) {
-                f32x16 &g = (K & 1 ? gk : gv)[db];
-                g = Mma<T>::mma(cf[K & 1][db], f, g);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        });
-        dma_wait();
-        __syncthreads();
+            for (int db = 0; db < DB; ++db) gv[db] = Mma<T>::mma(cg[db], pf, gv[db]);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) gk[db] = Mma<T>::mma(cq[db], df, gk[db]);
+        };
+        grads(std::integral_constant<int, 0>{});
+        pf = Mma<T>::pack(p), df = Mma<T>::pack(ds);
+        if (STAGGER) {
+            if (late) dma_wait();
+            meet();
+            if (!late && tn < nt) fetch(tn, s ^ 1);
+        }
+        bool u2 = true;
+        const int t2 = walk.next(tn + 1, u2);
+        peek(t2);
+        operands(0);
+        __builtin_amdgcn_sched_barrier(0);
+        products();
+        grads(std::integral_constant<int, 1>{});
+        pf = Mma<T>::pack(p), df = Mma<T>::pack(ds);
+        operands(16);
+        __builtin_amdgcn_sched_barrier(0);
+        products();
+        if (STAGGER) {
+            if (!late) dma_wait();
+            meet();
+        } else {
+            dma_wait();
+            __syncthreads();
+        }
         s ^= 1;
         t = tn, u = un, tn = t2, un = u2;
     }
+    if (STAGGER && !late) meet();
+    __syncthreads();
     if (QW > 1) {                                              // the row halves' sums, through the row buffers: gK, then gV
         float *red = reinterpret_cast<float *>(lrow[0]);
         auto join = [&](f32x16 (&g)[DB]) {
