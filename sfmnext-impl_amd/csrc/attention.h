@@ -32,7 +32,7 @@ struct AttnK {
     const int *prefix, *q_docs, *k_docs, *k_len;
     const int2 *doc_rng;                    // per tile of the looped-over side: smallest and largest document id
     int64_t qs[3], ks[3], vs[3], gos[3];
-    float scale_log2, cap_in, cap_out, scale;             // log2(e) scale; 2 log2(e) scale / cap, cap log2(e)
+    float scale_log2, cap_in, cap_arg, cap_out, scale;    // log2(e) scale; 2 log2(e) scale / cap, scale / cap, cap log2(e)
     unsigned g_magic;
     Deal deal;
     float unit_inv;                          // slopes are used in units of the raw score (1 / scale) or of tanh (1 / cap)
@@ -279,10 +279,12 @@ __device__ __forceinline__ float half_sum(float v) {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Scores in base 2: x = log2(e) (z - slope |pos - j|), z = scale q.k or c tanh(scale q.k / c).  tanh(u) = 1 - 2 / (e^{2u} + 1): one exponential and
-// one reciprocal; absolute error 1e-7, i.e. 1e-7 c of a score.  cap_in = 2 log2(e) scale / c, cap_out = c log2(e).
-template <bool CAP> __device__ __forceinline__ float tanh_of(float raw, float cap_in) {
-    return fmaf(-2.f, __builtin_amdgcn_rcpf(exp2_hw(raw * cap_in) + 1.f), 1.f);
+// tanh of a capped score (raw: the product before the scale).  16-bit types: 1 - 2 / (e^{2u} + 1), one exponential and one reciprocal; absolute error
+// 1e-7, i.e. 1e-7 of the cap in the score.  fp32 takes the library's tanh, whose error is relative: with a cap far above the scores the short
+// form would lose them (a cap of 10^4 leaves 6e-4 of a score), and the fp32 products are long enough to hide it.
+template <typename T> __device__ __forceinline__ float tanh_of(float raw, const AttnK &A) {
+    if constexpr (sizeof(T) == 4) return tanhf(raw * A.cap_arg);
+    else return fmaf(-2.f, __builtin_amdgcn_rcpf(exp2_hw(raw * A.cap_in) + 1.f), 1.f);
 }
 
 // what a row may see: keys j <= lim (lengths, causal order and prefix in one number), document equal

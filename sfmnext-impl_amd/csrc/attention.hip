@@ -58,7 +58,7 @@ template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    if (CAP) x[nb][r] = tanh_of<CAP>(x[nb][r], A.cap_in);
+                    if (CAP) x[nb][r] = tanh_of<T>(x[nb][r], A);
                     if (BIAS) x[nb][r] = fmaf(-slope, fabsf(d0 - (float)(nb * 32 + (r & 3) + 8 * (r >> 2))), x[nb][r]);
                 }
         }
@@ -437,16 +437,17 @@ int attn_check(const char *who, const sqd_attn_args *a) {
                   who, a->B, a->Sq, a->Sk, a->Hq, a->Hkv);
     SQD_CHECK_ARG(a->D >= 8 && a->D <= 128 && a->D % 8 == 0, "%s: %d features a head (a multiple of 8 up to 128)", who, a->D);
     SQD_CHECK_ARG(a->Sk < (1 << 24) && (int64_t)a->Sq * (a->Hq / a->Hkv) < (1 << 30) &&
-                      (int64_t)a->Sq * (a->Hq / a->Hkv) * (a->Hq / a->Hkv) < (1ll << 31) && (int64_t)a->B * a->Hkv < (1 << 24), "%s: too many tokens", who);
+                      (int64_t)a->Sq * (a->Hq / a->Hkv) * (a->Hq / a->Hkv) < (1ll << 31) && (int64_t)a->B * a->Hkv < (1 << 24) && a->B < 65536 && a->Hkv < 65536, "%s: too many tokens", who);
     SQD_CHECK_ARG(a->scale > 1e-30f && a->scale < 1e30f && a->softcap >= 0.f && a->softcap < 1e30f && (a->softcap == 0.f || a->softcap > 1e-30f), "%s: scale %g, cap %g", who, (double)a->scale, (double)a->softcap);
     SQD_CHECK_ARG(a->dtype >= SQD_F32 && a->dtype <= SQD_F16, "%s: element type %d", who, a->dtype);
     SQD_CHECK_ARG(!a->prefix || a->causal, "%s: a prefix needs the causal order", who);
     SQD_CHECK_ARG(!a->q_docs == !a->k_docs, "%s: documents of queries and keys come together", who);
     return SQD_OK;
 }
-int attn_check_tensor(const char *who, const char *name, const void *p, const int64_t *stride, int dtype) {
+// a tile of rows (up to 128 tokens, or 64 packed rows of G heads) is addressed by 32-bit offsets
+int attn_check_tensor(const char *who, const char *name, const void *p, const int64_t *stride, int heads, int dtype) {
     const int V = dtype == SQD_F32 ? 4 : 8;
-    SQD_CHECK_ARG(stride[1] >= 0 && stride[1] < (1 << 22) && stride[2] >= 0 && stride[2] < (1 << 22), "%s: token / head strides of %s: %lld, %lld", who, name,
+    SQD_CHECK_ARG(stride[1] >= 0 && stride[1] < (1 << 22) && stride[2] >= 0 && stride[2] * heads < (1 << 28), "%s: token / head strides of %s: %lld, %lld", who, name,
                   (long long)stride[1], (long long)stride[2]);
     SQD_CHECK_ARG(p && aligned16(p) && stride[0] % V == 0 && stride[1] % V == 0 && stride[2] % V == 0, "%s: %s must be 16-byte aligned, its strides too", who, name);
     return SQD_OK;
@@ -460,7 +461,7 @@ AttnK attn_kargs(const sqd_attn_args *a) {
     A.scale = a->scale;
     A.scale_log2 = (float)(a->scale * LOG2E);
     A.unit_inv = (float)(1.0 / (a->softcap > 0.f ? a->softcap : a->scale));
-    if (a->softcap > 0.f) A.cap_in = (float)(2.0 * LOG2E * a->scale / a->softcap), A.cap_out = (float)(a->softcap * LOG2E);
+    if (a->softcap > 0.f) A.cap_in = (float)(2.0 * LOG2E * a->scale / a->softcap), A.cap_arg = (float)((double)a->scale / a->softcap), A.cap_out = (float)(a->softcap * LOG2E);
     A.B = a->B, A.Sq = a->Sq, A.Sk = a->Sk, A.Hq = a->Hq, A.Hkv = a->Hkv, A.G = a->Hq / a->Hkv, A.D = a->D, A.causal = a->causal;
     A.g_magic = A.G == 1 ? 0u : (unsigned)(((1ull << 32) + A.G - 1) / A.G);
     return A;
@@ -481,10 +482,10 @@ extern "C" int sqd_attn_fwd(const sqd_attn_args *a) {
     if (int e = attn_check("sqd_attn_fwd", a)) return e;
     if ((int64_t)a->B * a->Sq == 0) return SQD_OK;
     SQD_CHECK_ARG(a->o && aligned16(a->o), "sqd_attn_fwd: o must be 16-byte aligned");
-    if (int e = attn_check_tensor("sqd_attn_fwd", "q", a->q, a->q_stride, a->dtype)) return e;
+    if (int e = attn_check_tensor("sqd_attn_fwd", "q", a->q, a->q_stride, a->Hq, a->dtype)) return e;
     if (a->Sk) {
-        if (int e = attn_check_tensor("sqd_attn_fwd", "k", a->k, a->k_stride, a->dtype)) return e;
-        if (int e = attn_check_tensor("sqd_attn_fwd", "v", a->v, a->v_stride, a->dtype)) return e;
+        if (int e = attn_check_tensor("sqd_attn_fwd", "k", a->k, a->k_stride, a->Hkv, a->dtype)) return e;
+        if (int e = attn_check_tensor("sqd_attn_fwd", "v", a->v, a->v_stride, a->Hkv, a->dtype)) return e;
     }
     const Split p = plan(a);
     SQD_CHECK_ARG(p.part_floats + p.lse_floats + p.rng_floats == 0 || (a->scratch && aligned16(a->scratch)), "sqd_attn_fwd: scratch missing");
@@ -498,6 +499,7 @@ extern "C" int sqd_attn_fwd(const sqd_attn_args *a) {
     SQD_CHECK_ARG(tiles < (1 << 24), "sqd_attn_fwd: too many tokens");
     A.deal = deal(A.B * A.Hkv, (int)tiles);
     const int64_t blocks = p.token ? tiles * A.B * A.Hkv : deal_blocks(A.deal);
+    SQD_CHECK_ARG(blocks < (1ll << 31), "sqd_attn_fwd: too many tokens");
     SQD_CHECK_ARG(blocks < (1ll << 31), "sqd_attn_fwd: too many tokens");
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);

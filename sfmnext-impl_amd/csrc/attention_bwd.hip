@@ -14,7 +14,7 @@
 
 namespace sqd {
 int attn_check(const char *who, const sqd_attn_args *a);
-int attn_check_tensor(const char *who, const char *name, const void *p, const int64_t *stride, int dtype);
+int attn_check_tensor(const char *who, const char *name, const void *p, const int64_t *stride, int heads, int dtype);
 AttnK attn_kargs(const sqd_attn_args *a);
 void attn_doc_ranges(const int *ids, int2 *out, int B, int S, int div, int span, int ntile, hipStream_t st);
 }  // namespace sqd
@@ -65,9 +65,9 @@ __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
 }
 
 // probability and score gradient (without the scale) of one pair, e = dP - delta; `see` false: zeros, whatever the products hold
-template <bool CAP, bool BIAS>
+template <typename T, bool CAP, bool BIAS>
 __device__ __forceinline__ void pair_grad(float raw, float e, float lse, float slope, float dist, const AttnK &A, bool see, float &p, float &ds) {
-    const float t = CAP ? tanh_of<CAP>(raw, A.cap_in) : raw, c = CAP ? A.cap_out : A.scale_log2;
+    const float t = CAP ? tanh_of<T>(raw, A) : raw, c = CAP ? A.cap_out : A.scale_log2;
     p = exp2_hw(fmaf(BIAS ? fmaf(-slope, fabsf(dist), t) : t, c, -lse));
     p = see ? p : 0.f;
     const float q = see && p < ONE_LESS ? p : 0.f;
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 
                 for (int e = 0; e < 4; ++e) {
                     const int r = (2 * H + r2) * 4 + e;
                     const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
-                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), p[r2 * 4 + e], ds[r2 * 4 + e]);
+                    pair_grad<T, CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), p[r2 * 4 + e], ds[r2 * 4 + e]);
                 }
             }
         };
@@ -470,7 +470,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
                     float p;
-                    pair_grad<CAP, BIAS>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
+                    pair_grad<T, CAP, BIAS>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
                 }
             }
         };
@@ -566,18 +566,19 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
     if (int e = attn_check(who, a)) return e;
     if (a->B == 0 || (a->Sq == 0 && a->Sk == 0)) return SQD_OK;
     if (a->Sq) {
-        if (int e = attn_check_tensor(who, "q", a->q, a->q_stride, a->dtype)) return e;
-        if (int e = attn_check_tensor(who, "go", a->go, a->go_stride, a->dtype)) return e;
-        SQD_CHECK_ARG(a->o && aligned16(a->o) && aligned16(a->o_low) && a->gq && aligned16(a->gq) && a->lse && a->scratch && aligned16(a->scratch),
+        if (int e = attn_check_tensor(who, "q", a->q, a->q_stride, a->Hq, a->dtype)) return e;
+        if (int e = attn_check_tensor(who, "go", a->go, a->go_stride, a->Hq, a->dtype)) return e;
+        SQD_CHECK_ARG(a->o && aligned16(a->o) && aligned16(a->o_low) && aligned16(a->gq) && a->lse && a->scratch && aligned16(a->scratch),
                       "%s: null or unaligned pointer", who);
     }
     if (a->Sk) {
-        if (int e = attn_check_tensor(who, "k", a->k, a->k_stride, a->dtype)) return e;
-        if (int e = attn_check_tensor(who, "v", a->v, a->v_stride, a->dtype)) return e;
-        SQD_CHECK_ARG(a->gk && a->gv && aligned16(a->gk) && aligned16(a->gv), "%s: null or unaligned pointer", who);
+        if (int e = attn_check_tensor(who, "k", a->k, a->k_stride, a->Hkv, a->dtype)) return e;
+        if (int e = attn_check_tensor(who, "v", a->v, a->v_stride, a->Hkv, a->dtype)) return e;
+        SQD_CHECK_ARG(!a->gk == !a->gv && aligned16(a->gk) && aligned16(a->gv), "%s: gk and gv come together, 16-byte aligned", who);
     }
     const BwdPlan p = bwd_plan(a);
     SQD_CHECK_ARG(p.rows < (1 << 28) && a->B < 65536 && a->Hkv < 65536, "%s: too many tokens", who);          // row records: 32-bit offsets between arrays
+    SQD_CHECK_ARG((int64_t)a->B * a->Hkv * 16 * ((a->Sk + 63) / 64 + 8) < (1ll << 31) && p.rows < (1ll << 31), "%s: too many tokens", who);
     AttnK A = attn_kargs(a);
     A.rows_padded = p.rows_padded;
     A.row_lse = a->scratch, A.row_delta = a->scratch + p.rows;
@@ -593,7 +594,7 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
         auto go = [&](auto dp, auto cap, auto bias) {
             constexpr int DP = decltype(dp)::value;
             constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
-            if (A.Sk) {
+            if (A.Sk && A.gk) {
                 AttnK K = A;
                 K.ntile = (A.Sk + 32 * p.kw - 1) / (32 * p.kw), K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
                 K.nsplit = p.k_split, K.part_a = a->scratch + p.parts, K.part_b = K.part_a + p.k_split * p.nk;
@@ -610,7 +611,7 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
                     hipLaunchKernelGGL((attn_parts_kernel<T>), g2, dim3(NT), 0, st, K.part_b, (T *)a->gv, p.nk / 4, K.nsplit);
                 }
             }
-            if (A.Sq) {
+            if (A.Sq && A.gq) {
                 AttnK Q = A;
                 Q.ntile = (int)(((int64_t)A.Sq * A.G + BM - 1) / BM), Q.doc_rng = k_rng, Q.ndoc_tiles = p.nk_tiles;
                 Q.nsplit = p.q_split, Q.part_a = a->scratch + p.parts;

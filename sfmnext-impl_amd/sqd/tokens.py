@@ -21,14 +21,14 @@ def on_device(t):
 
 
 def _rows16(t):
-    """t [B,S,H,D] with features dense, every other stride and the address in whole 16-byte pieces and the strides of tokens and heads below
-    2^22 elements: itself, or a copy"""
+    """t [B,S,H,D] with features dense, every other stride and the address in whole 16-byte pieces, the tokens' stride below 2^22 elements and
+    the heads' times their number below 2^28: itself, or a copy"""
     n = 16 // t.element_size()
     if t.numel() == 0:
         return t
     (b, s, h, e), (B, S, H, _) = t.stride(), t.shape
     if (e == 1 and t.data_ptr() % 16 == 0 and (B == 1 or b % n == 0) and (S == 1 or (s % n == 0 and 0 <= s < 1 << 22))
-            and (H == 1 or (h % n == 0 and 0 <= h < 1 << 22))):
+            and (H == 1 or (h % n == 0 and 0 <= h * H < 1 << 28))):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
@@ -198,8 +198,10 @@ class Attention(torch.autograd.Function):
         with on_device(q):
             go = _rows16(go)
             a = _attn_args(q, k, v, ctx.cfg, masks)
-            gq, gk, gv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
-            a.go, a.o, a.lse, a.gq, a.gk, a.gv = (t.data_ptr() for t in (go, o, lse, gq, gk, gv))
+            want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+            gq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if want_q else None
+            gk, gv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) if want_kv else None for t in (k, v))
+            a.go, a.o, a.lse, a.gq, a.gk, a.gv = (_ptr(t) for t in (go, o, lse, gq, gk, gv))
             a.go_stride[:] = _strides(go)
             a.o_low = _ptr(low)
             scratch = torch.empty(max(4, L.sqd_attn_bwd_scratch(ctypes.byref(a))), device=q.device, dtype=torch.float32)

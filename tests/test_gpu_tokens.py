@@ -251,6 +251,37 @@ def test_attention_hidden_places_hold_anything(dtype, junk):
             check(got, ref[name], ref[name + "_tol"], name)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cap", [0.5, 300.0, 30000.0])
+def test_attention_small_and_large_caps(cap, dtype):
+    """fp32 keeps scores far below the cap; the 16-bit types lose 4 2^-24 of the cap, which the bounds count"""
+    q, k, v, go, kw = _build(_case(2, 90, 90, 4, 2, 64, softcap=cap, causal=True), dtype)
+    ref = attention_ref(q, k, v, go=go, **kw)
+    d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    o = _ops().attention(*d, **_cuda(kw))
+    check(o, ref["o"], ref["o_tol"], "o")
+    if dtype == F32:           # the bound counts the short form's loss; fp32 must not have it: as exact as without a cap (64 roundings of 2^-24)
+        assert float((o.detach().cpu().double() - ref["o"]).norm() / ref["o"].norm()) < 64 * 2.0 ** -24
+    for name, got in zip(("gq", "gk", "gv"), torch.autograd.grad(o, d, go.cuda())):
+        check(got, ref[name], ref[name + "_tol"], name)
+
+
+def test_attention_frozen_inputs_and_expanded_gradients():
+    """only what requires a gradient gets one; keys and values expanded over the batch; the gradient of a sum is an expanded scalar"""
+    g = torch.Generator().manual_seed(2)
+    q, k, v = _rand(g, 3, 20, 4, 32), _rand(g, 1, 30, 2, 32), _rand(g, 1, 30, 2, 32)
+    ref = attention_ref(q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1), go=torch.ones_like(q))
+    dq, dk, dv = q.cuda().requires_grad_(True), k.cuda().requires_grad_(True), v.cuda().requires_grad_(True)
+    gq, gk, gv = torch.autograd.grad(_ops().attention(dq, dk.expand(3, -1, -1, -1), dv.expand(3, -1, -1, -1)).sum(), (dq, dk, dv))
+    check(gq, ref["gq"], ref["gq_tol"], "gq")
+    check(gk, ref["gk"].sum(0, keepdim=True), ref["gk_tol"].sum(0, keepdim=True) + 3 * 2.0 ** -24 * ref["gk"].abs().sum(0, keepdim=True), "gk")
+    check(gv, ref["gv"].sum(0, keepdim=True), ref["gv_tol"].sum(0, keepdim=True) + 3 * 2.0 ** -24 * ref["gv"].abs().sum(0, keepdim=True), "gv")
+    only, = torch.autograd.grad(_ops().attention(dq, k.cuda().expand(3, -1, -1, -1), v.cuda().expand(3, -1, -1, -1)).sum(), dq)
+    assert torch.equal(only, gq)
+    value, = torch.autograd.grad(_ops().attention(q.cuda(), k.cuda().expand(3, -1, -1, -1), dv.expand(3, -1, -1, -1)).sum(), dv)
+    assert torch.equal(value, gv)
+
+
 def test_attention_gradient_against_differences():
     """the directional derivative of sum(o go) in fp32 against central differences of the 64-bit definition (truncation h^2: 1e-8 relative)"""
     q, k, v, go, kw = _build(_case(1, 37, 37, 4, 2, 32, causal=True, prefix=[9], softcap=3.0, slopes=True), F32)
