@@ -201,8 +201,9 @@ template <typename T, int DP, int ROWS, int NTH> struct Stage {
 // acc[n] += sum over the features of frag_a(n, ks) x frag_b(ks): the LDS reads of BATCH steps are in flight while the step before multiplies.  Left
 // to itself the compiler reads one operand, waits for it and multiplies, and the LDS latency (some 130 cycles, against 32 of the
 // product) is paid in every step; the scheduling barriers keep the batches apart.
+// fp32, whose 16-feature step is eight long instructions, skips the steps past D (40 of 64 features: 3 steps of 4).
 template <typename T, int NACC, int KS, int BATCH, typename FA, typename FB>
-__device__ __forceinline__ void product(f32x16 (&acc)[NACC], FA &&frag_a, FB &&frag_b) {
+__device__ __forceinline__ void product(f32x16 (&acc)[NACC], int D, FA &&frag_a, FB &&frag_b) {
     constexpr int STEPS = NACC * KS / BATCH;
     typename Mma<T>::frag f[2][BATCH], g[2][BATCH];
     auto fetch = [&](auto st) {
@@ -221,7 +222,7 @@ __device__ __forceinline__ void product(f32x16 (&acc)[NACC], FA &&frag_a, FB &&f
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const int n = (S * BATCH + i) / KS;
-            acc[n] = Mma<T>::mma(f[S & 1][i], g[S & 1][i], acc[n]);
+            if (sizeof(T) == 2 || (S * BATCH + i) % KS * 16 < D) acc[n] = Mma<T>::mma(f[S & 1][i], g[S & 1][i], acc[n]);
         }
         __builtin_amdgcn_sched_barrier(0);
     });

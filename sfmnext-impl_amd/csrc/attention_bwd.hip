@@ -6,6 +6,9 @@
 // Two kernels and no atomics, so gradients repeat to the bit: one owns 128 keys and walks the rows that see them (gK, gV: four products of
 // the row tile), one owns 128 rows and walks their keys (gQ: three products).  Recomputing the scores in both costs 7 products where a single kernel
 // with atomic adds into gQ would take 5.
+// Measured: 2 x 3840 bf16 in 3 documents, 16 + 4 heads of 128, capped: gK gV 245 us (530 TFLOP/s), gQ 160 us (610); 12 x 480, 12 heads of 64, distance
+// bias: 55 and 33 us, row records 10 us; 2 x 1281 fp32, 8 + 4 heads of 40, causal, in 3 parts each: 101 and 77 us.  Bound by vector issue (some 12
+// operations and 1 to 3 exponentials or reciprocals a pair) and its overlap with the products.
 //
 // P within 2^-22 of one: every other key's P is below 2^-22 together and dP - delta is the difference of two equal numbers, rounding noise of
 // about that size; dS is taken as zero there (a row that sees ONE key has exactly no gradient for its scores).  P = 0 (masked): dS is zero
@@ -237,9 +240,9 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 
             for (int e = 0; e < 4; ++e) dp[4 * r4 + e] = -d[e];
         }
         constexpr int BATCH = KVL ? 2 : batch_of<T, L::KS>();
-        product<T, 1, L::KS, BATCH>(xs, [&](int, int ks) { return L::row_frag(lq, q0 + (lane & 31), ks, h); },
+        product<T, 1, L::KS, BATCH>(xs, A.D, [&](int, int ks) { return L::row_frag(lq, q0 + (lane & 31), ks, h); },
                                     [&](int ks) { return KVL ? L::row_frag(lk, kw * 32 + (lane & 31), ks, h) : kf[KVL ? 0 : ks]; });
-        product<T, 1, L::KS, BATCH>(dps, [&](int, int ks) { return L::row_frag(lg, q0 + (lane & 31), ks, h); },
+        product<T, 1, L::KS, BATCH>(dps, A.D, [&](int, int ks) { return L::row_frag(lg, q0 + (lane & 31), ks, h); },
                                     [&](int ks) { return KVL ? L::row_frag(lv, kw * 32 + (lane & 31), ks, h) : vf[KVL ? 0 : ks]; });
         // every row of the tile sees all of the wave's keys?  (limits do not fall with the row)
         const int R0 = t * QT + q0;
@@ -455,8 +458,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         const int j0 = t * KT;
         f32x16 xs[1] = {f32x16{}}, dps[1] = {minus_delta};
         f32x16 &x = xs[0], &dp = dps[0];
-        product<T, 1, L::KS, batch_of<T, L::KS>()>(xs, [&](int, int ks) { return L::row_frag(lk[s], lane & 31, ks, h); }, [&](int ks) { return qf[ks]; });
-        product<T, 1, L::KS, batch_of<T, L::KS>()>(dps, [&](int, int ks) { return L::row_frag(lv[s], lane & 31, ks, h); }, [&](int ks) { return gf[ks]; });
+        product<T, 1, L::KS, batch_of<T, L::KS>()>(xs, A.D, [&](int, int ks) { return L::row_frag(lk[s], lane & 31, ks, h); }, [&](int ks) { return qf[ks]; });
+        product<T, 1, L::KS, batch_of<T, L::KS>()>(dps, A.D, [&](int, int ks) { return L::row_frag(lv[s], lane & 31, ks, h); }, [&](int ks) { return gf[ks]; });
         const bool part = !u || __any(row.lim < j0 + KT - 1);
         float ds[16];
         const float d0 = (float)(row.pos - j0 - 4 * h);

@@ -8,6 +8,7 @@
 // workgroup takes a few tokens, computes their P angles once into LDS and applies them to all query and key heads: the trigonometry is
 // 1 / (Hq + Hk) of a per-element evaluation and the kernel stays HBM bound (every element read and written once, 16-byte pieces).  Queries and
 // keys go in one launch.
+// Measured: 40960 tokens, 16 + 4 heads of 128 bf16, 3 axes: 420 MB in 88 us = 4.8 TB/s (a plain copy: 5.0); 12 tokens 4.9 us, all latency.
 #include "sqd_vec.h"
 
 namespace {

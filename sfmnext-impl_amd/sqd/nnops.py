@@ -349,9 +349,9 @@ def _token_kernels():
 
 def _token_tensor(who, name, t, dim, like=None):
     """the checks that every tensor of a token operator passes; `like`: same element type and device"""
-    tokens = _token_kernels()
-    if isinstance(t, torch.Tensor) and t.dim() == dim and t.is_cuda and t.dtype in tokens.DTYPE and (
-            like is None or (t.dtype == like.dtype and t.device == like.device)):
+    tokens = _tokens or _token_kernels()
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in tokens.DTYPE and t.dim() == dim and (
+            like is None or (t.dtype == like.dtype and t.get_device() == like.get_device())):
         return
     if not isinstance(t, torch.Tensor) or t.dim() != dim:
         raise RuntimeError("sqd: %s: %s must be a tensor of %d dimensions" % (who, name, dim))
@@ -359,12 +359,11 @@ def _token_tensor(who, name, t, dim, like=None):
         raise RuntimeError("sqd: %s must run on the MI355X (HIP) device: %s is on %s; there is no CPU fallback" % (who, name, t.device))
     if t.dtype not in tokens.DTYPE:
         raise RuntimeError("sqd: %s: %s is %s (float32, bfloat16 or float16)" % (who, name, t.dtype))
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise RuntimeError("sqd: %s: %s is %s on %s, the first tensor %s on %s" % (who, name, t.dtype, t.device, like.dtype, like.device))
+    raise RuntimeError("sqd: %s: %s is %s on %s, the first tensor %s on %s" % (who, name, t.dtype, t.device, like.dtype, like.device))
 
 
 def _index_tensor(who, name, t, shape, device, types):
-    if not isinstance(t, torch.Tensor) or t.dtype not in types or t.device != device or tuple(t.shape) != tuple(shape):
+    if not isinstance(t, torch.Tensor) or t.dtype not in types or t.device != device or t.shape != shape:
         raise RuntimeError("sqd: %s: %s must be %s of shape %s on %s" % (who, name, " | ".join(str(d) for d in types), tuple(shape), device))
     return t.contiguous()
 
@@ -387,7 +386,7 @@ def rms_norm_residual(x, weight, residual=None, eps=1e-6):
             raise RuntimeError("sqd: %s: residual %s against x %s" % (who, tuple(residual.shape), tuple(x.shape)))
     if not eps >= 0.0:
         raise RuntimeError("sqd: %s: eps = %r" % (who, eps))
-    tokens = _token_kernels()
+    tokens = _tokens
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         out = tokens.RmsNormResidual.apply(x, weight, residual, float(eps))
         return out if residual is not None else (out, x)
@@ -427,7 +426,7 @@ def rotary_axes(q, k, positions, freq, pairs, interleaved=False):
         raise RuntimeError("sqd: %s: positions must be [S,A] or [B,S,A]" % who)
     positions = _index_tensor(who, "positions", positions, ((S,) if positions.dim() == 2 else (B, S)) + (len(pairs),), q.device, (torch.int32, torch.int64))
     freq = _index_tensor(who, "freq", freq, (P,), q.device, (torch.float64,))
-    tokens = _token_kernels()
+    tokens = _tokens
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = tokens.RotaryAxes.apply(q, k, positions, freq, pairs, int(bool(interleaved)))
         return out if k is not None else (out, None)
@@ -476,7 +475,7 @@ def attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefi
         k_docs = _index_tensor(who, "k_docs", k_docs, (B, Sk), q.device, i32)
     if k_len is not None:
         k_len = _index_tensor(who, "k_len", k_len, (B,), q.device, i32)
-    tokens = _token_kernels()
+    tokens = _tokens
     cfg, masks = (scale, softcap, int(bool(causal))), (slopes, prefix, q_docs, k_docs, k_len)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return tokens.Attention.apply(q, k, v, cfg, *masks)

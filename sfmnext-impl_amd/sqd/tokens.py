@@ -13,11 +13,12 @@ from .ops import _ptr, _stream
 
 DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # SQD_F32 | SQD_BF16 | SQD_F16
 _SAME = contextlib.nullcontext()
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def on_device(t):
     """the launches of a call go to the device its tensors live on, whichever device is current"""
-    return _SAME if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _SAME if t.get_device() == _current() else torch.cuda.device(t.device)
 
 
 def _rows16(t):
@@ -36,7 +37,8 @@ def _rows16(t):
 
 def _strides(t):
     """element strides of batch, token and head; 0 where there is one only"""
-    return [s if d > 1 else 0 for s, d in zip(t.stride()[:3], t.shape[:3])]
+    (b, s, h, _), (B, S, H, _) = t.stride(), t.shape
+    return (b if B > 1 else 0, s if S > 1 else 0, h if H > 1 else 0)
 
 
 # ------------------------------------------------------------------------------------------------------------------ residual RMS norm
@@ -100,17 +102,11 @@ def _rotate(q, k, pos, freq, pairs, interleaved, inverse):
     B, S, Hq, D = q.shape
     with on_device(q):
         q, k = _rows16(q), _rows16(k) if k is not None else None
-        a = RotaryArgs()
         qo = torch.empty((B, S, Hq, D), device=q.device, dtype=q.dtype)
         ko = torch.empty(k.shape, device=q.device, dtype=q.dtype) if k is not None else None
-        a.q, a.q_out, a.q_stride[:] = q.data_ptr(), qo.data_ptr(), _strides(q)
-        if k is not None:
-            a.k, a.k_out, a.k_stride[:], a.Hk = k.data_ptr(), ko.data_ptr(), _strides(k), k.shape[2]
-        a.pos, a.freq, a.pos_bytes, a.axes = pos.data_ptr(), freq.data_ptr(), pos.element_size(), len(pairs)
-        a.pos_batch_stride = pos.stride(0) if pos.dim() == 3 else 0
-        a.pairs[:len(pairs)] = pairs
-        a.B, a.S, a.Hq, a.D, a.interleaved, a.inverse, a.dtype = B, S, Hq, D, interleaved, inverse, DTYPE[q.dtype]
-        a.stream = _stream()
+        a = RotaryArgs(q.data_ptr(), _ptr(k), qo.data_ptr(), _ptr(ko), pos.data_ptr(), freq.data_ptr(), _stream(), _strides(q),
+                       _strides(k) if k is not None else (0, 0, 0), pos.stride(0) if pos.dim() == 3 else 0, pairs, B, S, Hq,
+                       k.shape[2] if k is not None else 0, D, len(pairs), pos.element_size(), interleaved, inverse, DTYPE[q.dtype])
         _l.check(_l.lib().sqd_rotary_axes(ctypes.byref(a)), "rotary_axes")
     return qo, ko
 
@@ -149,27 +145,26 @@ class AttnArgs(ctypes.Structure):
                 ("B", _I), ("Sq", _I), ("Sk", _I), ("Hq", _I), ("Hkv", _I), ("D", _I), ("causal", _I), ("dtype", _I)]
 
 
-def _attn_args(q, k, v, cfg, masks):
-    a = AttnArgs()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
-    a.B, a.Sq, a.Hq, a.D = q.shape
-    a.Sk, a.Hkv = k.shape[1], k.shape[2]
-    a.scale, a.softcap, a.causal = cfg
-    a.slopes, a.prefix, a.q_docs, a.k_docs, a.k_len = [_ptr(m) for m in masks]
-    a.dtype = DTYPE[q.dtype]
-    a.stream = _stream()
-    return a
+def _attn_args(q, k, v, cfg, masks, out, go=None):
+    """the argument block; out = (o, o_low, gq, gk, gv, lse, scratch), masks = (slopes, prefix, q_docs, k_docs, k_len)"""
+    B, Sq, Hq, D = q.shape
+    o, o_low, gq, gk, gv, lse, scratch = [_ptr(t) for t in out]
+    return AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(go), o, o_low, gq, gk, gv, lse, scratch, *[_ptr(m) for m in masks], _stream(),
+                    _strides(q), _strides(k), _strides(v), _strides(go) if go is not None else (0, 0, 0), cfg[0], cfg[1], B, Sq, k.shape[1], Hq,
+                    k.shape[2], D, cfg[2], DTYPE[q.dtype])
 
 
 def attn_fwd(q, k, v, cfg, masks, want_lse):
-    """-> o [B,Sq,Hq,D]; for the backward (want_lse): what its rounding left (16-bit types) and lse [B,Hkv,Sq*G]; cfg = (scale, softcap, causal), masks = (slopes, prefix, q_docs, k_docs, k_len)"""
+    """-> o [B,Sq,Hq,D]; for the backward (want_lse): what its rounding left (16-bit types) and lse [B,Hkv,Sq*G], else None.
+    cfg = (scale, softcap, causal), masks = (slopes, prefix, q_docs, k_docs, k_len)"""
     L = _l.lib()
-    a = _attn_args(q, k, v, cfg, masks)
     o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty((q.shape[0], k.shape[2], q.shape[1] * (q.shape[2] // k.shape[2])), device=q.device, dtype=torch.float32) if want_lse else None
-    low = torch.empty_like(o) if want_lse and o.dtype != torch.float32 else None
-    a.o, a.o_low, a.lse = o.data_ptr(), _ptr(low), _ptr(lse)
+    low = lse = None
+    if want_lse:
+        lse = torch.empty((q.shape[0], k.shape[2], q.shape[1] * (q.shape[2] // k.shape[2])), device=q.device, dtype=torch.float32)
+        if o.dtype != torch.float32:
+            low = torch.empty_like(o)
+    a = _attn_args(q, k, v, cfg, masks, (o, low, None, None, None, lse, None))
     n = L.sqd_attn_fwd_scratch(ctypes.byref(a))
     if n > 0:
         scratch = torch.empty(n, device=q.device, dtype=torch.float32)
@@ -197,13 +192,10 @@ class Attention(torch.autograd.Function):
         L = _l.lib()
         with on_device(q):
             go = _rows16(go)
-            a = _attn_args(q, k, v, ctx.cfg, masks)
             want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
             gq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if want_q else None
             gk, gv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) if want_kv else None for t in (k, v))
-            a.go, a.o, a.lse, a.gq, a.gk, a.gv = (_ptr(t) for t in (go, o, lse, gq, gk, gv))
-            a.go_stride[:] = _strides(go)
-            a.o_low = _ptr(low)
+            a = _attn_args(q, k, v, ctx.cfg, masks, (o, low, gq, gk, gv, lse, None), go)
             scratch = torch.empty(max(4, L.sqd_attn_bwd_scratch(ctypes.byref(a))), device=q.device, dtype=torch.float32)
             a.scratch = scratch.data_ptr()
             _l.check(L.sqd_attn_bwd(ctypes.byref(a)), "attn_bwd")
