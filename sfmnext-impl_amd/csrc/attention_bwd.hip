@@ -7,7 +7,7 @@
 // the row tile), one owns 128 rows and walks their keys (gQ: three products).  Recomputing the scores in both costs 7 products where a single kernel
 // with atomic adds into gQ would take 5.
 // Measured: 2 x 3840 bf16 in 3 documents, 16 + 4 heads of 128, capped: gK gV 245 us (530 TFLOP/s), gQ 160 us (610); 12 x 480, 12 heads of 64, distance
-// bias: 55 and 33 us, row records 10 us; 2 x 1281 fp32, 8 + 4 heads of 40, causal, in 3 parts each: 101 and 77 us.  Bound by vector issue (some 12
+// bias: 46 and 33 us, row records 10 us; 2 x 1281 fp32, 8 + 4 heads of 40, causal, in 3 parts each: 101 and 77 us.  Bound by vector issue (some 12
 // operations and 1 to 3 exponentials or reciprocals a pair) and its overlap with the products.
 //
 // P within 2^-22 of one: every other key's P is below 2^-22 together and dP - delta is the difference of two equal numbers, rounding noise of
@@ -80,9 +80,9 @@ __device__ __forceinline__ void pair_grad(float raw, float e, float lse, float s
 
 // KW waves side by side on 32 keys each, times QW on the 32-row parts of a row tile.  A wave needs its gK and gV sums (64 registers each at 128
 // features) and the operands of its keys (32 + 32): with those in registers one wave fits a SIMD and every latency is paid.  KVL keeps the keys'
-// operands in LDS instead: 8 waves of 256 registers, two a SIMD.
+// operands in LDS instead: at 128 features 8 waves of 256 registers, two a SIMD; at 64 three workgroups of 4 waves a CU.
 template <typename T, int DP, int KW, int QW, bool KVL, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_kernel(AttnK A) {
+__global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_kernel(AttnK A) {
     constexpr int NT = 64 * KW * QW, QT = 32 * QW, DB = DP / 32;
     typedef Tile<T, DP> L;
     typedef typename L::frag frag;
@@ -537,11 +537,12 @@ int parts_of(int64_t blocks, int64_t tiles) {
 BwdPlan bwd_plan(const sqd_attn_args *a) {
     BwdPlan p{};
     const int G = a->Hq / a->Hkv;
-    // keys and row parts of a workgroup: 128 x 2 with 8 waves where that fits (16-bit types past 64 features) and gives most CUs a workgroup; else 4
-    // waves, 64 x 2 while 128 x 1 would leave CUs idle or a last round nearly empty
+    // keys and row parts of a workgroup.  128 x 2 with 8 waves where that fits (16-bit types past 64 features) and most CUs get one.  Else 4 waves: 64
+    // x 2 makes twice the workgroups of 128 x 1, which wins once those fill the card by themselves (bf16, 64 features: 576 workgroups of 128 keys
+    // 47 us against 56, 480: 58 against 54; fp32: 768: 482 against 500, 576: 259 against 242)
     const int64_t wide = (int64_t)((a->Sk + 127) / 128) * a->B * a->Hkv;
     if (a->dtype != SQD_F32 && a->D > 64 && wide >= 192) p.kw = 4, p.qw = 2;
-    else if (wide < 1024) p.kw = 2, p.qw = 2;
+    else if (wide < (a->dtype == SQD_F32 ? 768 : 512)) p.kw = 2, p.qw = 2;
     else p.kw = 4, p.qw = 1;
     const int QT = 32 * p.qw;
     p.rows_padded = (a->Sq * G + 63) / 64 * 64;
@@ -607,7 +608,7 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
                     if (p.kw == 4 && p.qw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 2, true, CAP, BIAS>), grid, dim3(512), 0, st, K);
                 }
                 if (p.kw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 2, 2, false, CAP, BIAS>), grid, dim3(NT), 0, st, K);
-                else if (p.qw == 1) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 1, false, CAP, BIAS>), grid, dim3(NT), 0, st, K);
+                else if (p.qw == 1) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 1, (DP * sizeof(T) == 128), CAP, BIAS>), grid, dim3(NT), 0, st, K);
                 if (K.nsplit > 1) {                                // (parts of dK, dV are joined before the scratch holds dQ's)
                     const dim3 g2((unsigned)((p.nk / 4 + NT - 1) / NT));
                     hipLaunchKernelGGL((attn_parts_kernel<T>), g2, dim3(NT), 0, st, K.part_a, (T *)a->gk, p.nk / 4, K.nsplit);

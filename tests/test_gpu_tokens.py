@@ -178,6 +178,7 @@ WIDE = [
     (_case(8, 200, 200, 16, 16, 128, docs=(3, 17), softcap=20.0), BF16), (_case(8, 150, 290, 8, 8, 96, causal=True, k_len=[290, 2, 150, 149, 77, 200, 13, 290]), F16),
     (_case(6, 129, 129, 70, 70, 16, causal=True, prefix=[0, 1, 50, 129, 200, 128]), BF16), (_case(6, 140, 140, 65, 65, 8, slopes=True), F32),
     (_case(1, 1100, 1100, 1, 1, 64, causal=True), BF16), (_case(1, 901, 1203, 3, 1, 40, softcap=9.0, causal=True, prefix=[300]), F32),
+    (_case(8, 130, 130, 40, 40, 64, slopes=True, docs=(2, 9)), BF16), (_case(4, 200, 260, 64, 64, 48, causal=True, softcap=8.0), F16),
     (_case(3, 700, 700, 2, 1, 128, docs=(4, 90), slopes=True), F16), (_case(1, 700, 701, 5, 5, 64, causal=True, k_len=[640]), BF16),
 ]
 
