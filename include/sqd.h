@@ -803,13 +803,12 @@ int sqd_rotary_axes(const sqd_rotary_args *a);
  *   pos_i = i + n - Sq, n = k_len[b] (or NULL: Sk): the queries are the LAST Sq of n positions.  Keys j >= n are hidden.
  *   causal: j <= pos_i is seen; prefix [B] (or NULL; causal only): j < prefix[b] too
  *   q_docs [B,Sq], k_docs [B,Sk] (both or neither): i sees j where the two are equal and >= 0 (negative: padding)
- * A row that sees no key gets zeros.  Keys that no query may see (j >= n, negative document) are read as zeros, whatever they hold.
+ * A row that sees no key gets zeros, whatever it holds.  Keys j >= n and keys of a negative document are never read.
  *   fwd: o [B,Sq,Hq,D] dense; lse [B,Hkv,Sq*G] (G = Hq/Hkv, row i*G + g; log2 of the softmax sum in base-2 scores, +inf for an empty row)
  *        or NULL; o_low (16-bit types, or NULL): what o's rounding left, for the backward.  scratch: sqd_attn_fwd_scratch(a) floats (keys
  *        split over workgroups when there are few rows; 0: none needed).
- *   bwd: q, k, v, o, o_low (or NULL: gradients lose a little), lse as of the forward, go [B,Sq,Hq,D] with its own strides -> gq [B,Sq,Hq,D] (NULL: not wanted),
- *        gk, gv [B,Sk,Hkv,D] (both or neither) dense;
- *        scratch: sqd_attn_bwd_scratch(a) floats.                                                                                    */
+ *   bwd: q, k, v, o, o_low (or NULL: gradients lose a little), lse as of the forward, go [B,Sq,Hq,D] with its own strides ->
+ *        gq [B,Sq,Hq,D] (NULL: not wanted), gk, gv [B,Sk,Hkv,D] (both or neither), dense;  scratch: sqd_attn_bwd_scratch(a) floats.                                                                                    */
 typedef struct sqd_attn_args {
     const void *q, *k, *v, *go;
     void *o, *o_low, *gq, *gk, *gv;

@@ -56,9 +56,10 @@ __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
     for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 16);
     if ((threadIdx.x & 15) == 0) {
         const int64_t bh = (int64_t)b * A.Hkv + hk, at = bh * A.rows_padded + R;
+        const float lse = row.lim >= 0 ? A.lse[bh * RT + R] : INFINITY;
         A.row_delta[at] = s;
-        A.row_lse[at] = row.lim >= 0 ? A.lse[bh * RT + R] : INFINITY;
-        A.row_lim[at] = row.lim;
+        A.row_lse[at] = lse;
+        A.row_lim[at] = lse == INFINITY ? -1 : row.lim;        // documents may hide every key of a row that its limit allows
         A.row_doc[at] = row.qd;
         if (A.slopes) {
             A.row_pos[at] = (float)row.pos;

@@ -442,9 +442,8 @@ def attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefi
     than its contents), keys from n on are hidden.  causal: query i sees j <= pos_i, and j < prefix[b] (int32 [B]) whatever its own position.
     q_docs [B,Sq], k_docs [B,Sk] (int32; k_docs defaults to q_docs where Sq = Sk): i sees j of its own document; a negative document is padding.
 
-    A query that sees no key gets zeros, and zero gradients.  Keys behind n, padding keys and padding queries may hold anything.  Elsewhere a
-    masked product is zero times the value, as in any matrix product: an infinite or NaN value that SOME query of the call sees may reach
-    others.  Differentiable in q, k, v; slopes are constants (refused if they require a gradient)."""
+    A query that sees no key gets zeros, and zero gradients.  It may hold anything, and so may keys behind n and padding keys.  Elsewhere a masked
+    product is zero times the value, as in any matrix product: infinite or NaN values may reach queries that mask them.  Differentiable in q, k, v; slopes are constants (refused if they require a gradient)."""
     who = "attention"
     _token_tensor(who, "q", q, 4), _token_tensor(who, "k", k, 4, q), _token_tensor(who, "v", v, 4, q)
     B, Sq, Hq, D = q.shape

@@ -283,6 +283,20 @@ def test_attention_frozen_inputs_and_expanded_gradients():
     assert torch.equal(value, gv)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_queries_of_a_document_without_keys_hold_anything(dtype):
+    q, k, v, go, kw = _build(_case(2, 90, 150, 4, 2, 64, docs_random=True), dtype)
+    kw["k_docs"] = torch.where(kw["k_docs"] == 3, 4, kw["k_docs"])                    # nobody has document 3
+    lost = (kw["q_docs"] == 3) | (kw["q_docs"] < 0)
+    ref = attention_ref(q, k, v, go=go, **kw)
+    q[lost], go[lost] = math.nan, math.inf
+    d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    o = _ops().attention(*d, **_cuda(kw))
+    check(o, ref["o"], ref["o_tol"], "o")
+    for name, got in zip(("gq", "gk", "gv"), torch.autograd.grad(o, d, go.cuda())):
+        check(got, ref[name], ref[name + "_tol"], name)
+
+
 def test_attention_gradient_against_differences():
     """the directional derivative of sum(o go) in fp32 against central differences of the 64-bit definition (truncation h^2: 1e-8 relative)"""
     q, k, v, go, kw = _build(_case(1, 37, 37, 4, 2, 32, causal=True, prefix=[9], softcap=3.0, slopes=True), F32)
