@@ -141,7 +141,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
     const int split = w % A.nsplit, tile = A.ntile - 1 - w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;        // the longest causal rows first
     const int RT = A.Sq * A.G, row0 = tile * BM;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
-    const int prefix = A.prefix ? A.prefix[b] : 0;
+    const int prefix = A.prefix ? max(A.prefix[b], 0) : 0;
     const int R = row0 + wave * 32 + (lane & 31);               // this lane's row (both half-waves hold the same 32)
     const RowOf row = row_of(A, b, R, RT, len, prefix);
     clear_lds<NT>(lk[0], 2 * S::BYTES, tid);
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
     const int groups = A.B * A.Hkv, split = blockIdx.x / groups, bh = blockIdx.x - split * groups, hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, R = lane & 31;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
-    const int prefix = A.prefix ? A.prefix[b] : 0;
+    const int prefix = A.prefix ? max(A.prefix[b], 0) : 0;
     const RowOf row = row_of(A, b, R, RT, len, prefix);
     clear_lds<64>(buf[wave], 4 * S::BYTES, lane);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -508,7 +508,6 @@ extern "C" int sqd_attn_fwd(const sqd_attn_args *a) {
     SQD_CHECK_ARG(tiles < (1 << 24), "sqd_attn_fwd: too many tokens");
     A.deal = deal(A.B * A.Hkv, (int)tiles);
     const int64_t blocks = p.token ? tiles * A.B * A.Hkv : deal_blocks(A.deal);
-    SQD_CHECK_ARG(blocks < (1ll << 31), "sqd_attn_fwd: too many tokens");
     SQD_CHECK_ARG(blocks < (1ll << 31), "sqd_attn_fwd: too many tokens");
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
     const int RT = A.Sq * A.G, c = (threadIdx.x & 15) * 8, hk = blockIdx.y, b = blockIdx.z;
     const int R = blockIdx.x * (NT / 16) + (threadIdx.x >> 4);
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
-    const RowOf row = row_of(A, b, R, RT, len, A.prefix ? A.prefix[b] : 0);
+    const RowOf row = row_of(A, b, R, RT, len, A.prefix ? max(A.prefix[b], 0) : 0);
     const int hq = hk * A.G + row.g;
     float s = 0.f;
     if (c < A.D && row.lim >= 0) {
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
     const int tile = u0 / A.nsplit, split = u0 - tile * A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, j0 = tile * 32 * KW, jl = j0 + kw * 32 + (lane & 31);
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk, off = len - A.Sq;
-    const int prefix = A.prefix ? A.prefix[b] : 0;
+    const int prefix = A.prefix ? max(A.prefix[b], 0) : 0;
     const int *qdoc = A.q_docs ? A.q_docs + (int64_t)b * A.Sq : nullptr;
     const bool docs = qdoc != nullptr;
     int kd = -3;
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     const int split = w % A.nsplit, tile = A.ntile - 1 - w / A.nsplit, hk = bh % A.Hkv, b = bh / A.Hkv;
     const int RT = A.Sq * A.G, row0 = tile * BM;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
-    const int prefix = A.prefix ? A.prefix[b] : 0;
+    const int prefix = A.prefix ? max(A.prefix[b], 0) : 0;
     const int R = row0 + wave * 32 + (lane & 31);
     const RowOf row = row_of(A, b, R, RT, len, prefix);
     clear_lds<NT>(lk[0], 2 * S::BYTES, tid);

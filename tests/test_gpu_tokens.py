@@ -297,6 +297,21 @@ def test_attention_queries_of_a_document_without_keys_hold_anything(dtype):
         check(got, ref[name], ref[name + "_tol"], name)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_negative_prefix_is_no_prefix(dtype):
+    """down to the type's lowest value"""
+    q, k, v, go, _ = _build(_case(3, 70, 90, 4, 2, 64, causal=True), dtype)
+    lens = torch.tensor([90, 40, 90], dtype=torch.int32)
+    prefix = torch.tensor([-2 ** 31, -2 ** 31, -5], dtype=torch.int32)
+    ref = attention_ref(q, k, v, go=go, causal=True, k_len=lens, prefix=torch.zeros_like(prefix))
+    d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    o = _ops().attention(*d, causal=True, k_len=lens.cuda(), prefix=prefix.cuda())
+    check(o, ref["o"], ref["o_tol"], "o")
+    for name, got in zip(("gq", "gk", "gv"), torch.autograd.grad(o, d, go.cuda())):
+        check(got, ref[name], ref[name + "_tol"], name)
+    check(_ops().attention(q[:1, -1:].cuda(), k[:1].cuda(), v[:1].cuda(), causal=True, prefix=prefix[:1].cuda()), ref["o"][:1, -1:], ref["o_tol"][:1, -1:], "token")
+
+
 def test_attention_gradient_against_differences():
     """the directional derivative of sum(o go) in fp32 against central differences of the 64-bit definition (truncation h^2: 1e-8 relative)"""
     q, k, v, go, kw = _build(_case(1, 37, 37, 4, 2, 32, causal=True, prefix=[9], softcap=3.0, slopes=True), F32)
