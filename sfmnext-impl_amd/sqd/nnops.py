@@ -410,7 +410,7 @@ def rotary_axes(q, k, positions, freq, pairs, interleaved=False):
     """Rotary positions over 1 to 4 axes (time, row, column).  q [B,S,Hq,D], k [B,S,Hk,D] or None; positions [S,A] or [B,S,A] (int32 | int64, any
     sign and size); pairs: for each axis how many of the head's rotation pairs turn with it, P = sum(pairs) <= D / 2 in order; freq [P] float64
     (rotary_frequencies).  Pair p is (p, p + P), interleaved: (2p, 2p + 1); features behind 2P pass unchanged.  -> new dense q, k.
-    Angles are taken in 64 bits.  Differentiable in q and k."""
+    Angles are taken in 64 bits.  Differentiable in q and k; freq is a constant (refused if it requires a gradient)."""
     who = "rotary_axes"
     _token_tensor(who, "q", q, 4)
     B, S, Hq, D = q.shape
@@ -426,6 +426,8 @@ def rotary_axes(q, k, positions, freq, pairs, interleaved=False):
         raise RuntimeError("sqd: %s: positions must be [S,A] or [B,S,A]" % who)
     positions = _index_tensor(who, "positions", positions, ((S,) if positions.dim() == 2 else (B, S)) + (len(pairs),), q.device, (torch.int32, torch.int64))
     freq = _index_tensor(who, "freq", freq, (P,), q.device, (torch.float64,))
+    if freq.requires_grad:
+        raise RuntimeError("sqd: %s: the frequencies are constants; no gradient is computed for them" % who)
     tokens = _tokens
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = tokens.RotaryAxes.apply(q, k, positions, freq, pairs, int(bool(interleaved)))
@@ -457,9 +459,9 @@ def attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefi
     if not 0.0 < scale < 3e38 or not 0.0 <= softcap < 3e38:
         raise RuntimeError("sqd: %s: scale %r must be positive, softcap %r not negative" % (who, scale, softcap))
     if slopes is not None:
+        slopes = _index_tensor(who, "slopes", slopes, (Hq,), q.device, (torch.float32,))
         if slopes.requires_grad:
             raise RuntimeError("sqd: %s: the slopes of the distance bias are constants; no gradient is computed for them" % who)
-        slopes = _index_tensor(who, "slopes", slopes, (Hq,), q.device, (torch.float32,))
     i32 = (torch.int32,)
     if prefix is not None:
         if not causal:

@@ -486,6 +486,16 @@ def test_refusals():
             pytest.fail("call %d was not refused" % n)
 
 
+def test_constants_that_want_a_gradient_are_refused():
+    ops = _ops()
+    q = torch.zeros(2, 4, 4, 16, device="cuda")
+    pos, freq = torch.zeros(4, 1, device="cuda", dtype=torch.int32), torch.zeros(8, device="cuda", dtype=torch.float64, requires_grad=True)
+    for call in (lambda: ops.rotary_axes(q, None, pos, freq, (8,)), lambda: ops.rotary_axes(q.clone().requires_grad_(True), q, pos, freq, (8,)),
+                 lambda: ops.attention(q, q, q, slopes=[0.5] * 4), lambda: ops.attention(q, q, q, slopes=torch.zeros(4, device="cuda", requires_grad=True))):
+        with pytest.raises(RuntimeError, match="sqd: "):
+            call()
+
+
 def test_second_derivatives_are_refused():
     ops = _ops()
     x = torch.randn(4, 8, device="cuda", requires_grad=True)
