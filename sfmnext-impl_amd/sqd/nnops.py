@@ -352,6 +352,8 @@ def _token_tensor(who, name, t, dim, like=None):
     tokens = _tokens or _token_kernels()
     if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in tokens.DTYPE and t.dim() == dim and (
             like is None or (t.dtype == like.dtype and t.get_device() == like.get_device())):
+        if t.numel() >> 31 and max(t.shape) >> 31:         # the argument blocks hold 32-bit sizes
+            raise RuntimeError("sqd: %s: %s %s: every size must be below 2^31" % (who, name, tuple(t.shape)))
         return
     if not isinstance(t, torch.Tensor) or t.dim() != dim:
         raise RuntimeError("sqd: %s: %s must be a tensor of %d dimensions" % (who, name, dim))

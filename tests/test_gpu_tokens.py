@@ -496,6 +496,20 @@ def test_constants_that_want_a_gradient_are_refused():
             call()
 
 
+def test_sizes_past_32_bits_are_refused():
+    """expanded tensors (no memory behind the sizes): they must not be taken modulo 2^32"""
+    ops = _ops()
+    n = 2 ** 32 + 4
+    row = torch.zeros(1, device="cuda", dtype=F16)
+    q, few = torch.zeros(1, 1, 1, 16, device="cuda", dtype=F16), torch.zeros(1, 4, 1, 16, device="cuda", dtype=F16)
+    pos, freq = torch.zeros(1, 1, device="cuda", dtype=torch.int32), torch.zeros(8, device="cuda", dtype=torch.float64)
+    long = q.expand(1, n, 1, 16)
+    for call in (lambda: ops.rms_norm_residual(row.expand(n), row.expand(n)), lambda: ops.rotary_axes(long, None, pos.expand(n, 1), freq, (8,)),
+                 lambda: ops.attention(long, few, few), lambda: ops.attention(few, long, long), lambda: ops.attention(q.expand(n, 1, 1, 16), q, q)):
+        with pytest.raises(RuntimeError, match="sqd: "):
+            call()
+
+
 def test_second_derivatives_are_refused():
     ops = _ops()
     x = torch.randn(4, 8, device="cuda", requires_grad=True)
