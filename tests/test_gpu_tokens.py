@@ -172,6 +172,23 @@ def test_attention(n, dtype):
         assert torch.equal(_ops().attention(*d, **_cuda(kw)), o)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("extra", [{}, {"softcap": 20.0}, {"slopes": True}, {"softcap": 6.0, "slopes": True}])
+def test_attention_documents_with_every_score(extra, D, dtype):
+    """documents against each kernel (few rows, many) and each form of the scores; whole tiles of one document, so that every key of a tile counts"""
+    cases = [_case(2, 32, 32, 1, 1, D, docs=(1, 0), **extra), _case(2, 32, 32, 2, 2, D, docs=(5, 4), **extra), _case(1, 8, 8, 12, 3, D, docs=(2, 1), **extra),
+             _case(2, 5, 330, 4, 2, D, docs_random=True, **extra), _case(2, 96, 96, 2, 1, D, docs=(1, 0), **extra), _case(1, 200, 200, 2, 2, D, docs=(3, 8), causal=True, **extra)]
+    for c in cases:
+        q, k, v, go, kw = _build(c, dtype)
+        ref = attention_ref(q, k, v, go=go, **kw)
+        d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+        o = _ops().attention(*d, **_cuda(kw))
+        check(o, ref["o"], ref["o_tol"], "o %s" % c)
+        for name, got in zip(("gq", "gk", "gv"), torch.autograd.grad(o, d, go.cuda())):
+            check(got, ref[name], ref[name + "_tol"], "%s %s" % (name, c))
+
+
 # the variants a size selects: 128-key workgroups of 8 and of 4 waves, keys or rows split over workgroups (few heads, long sequences), key heads that
 # share an XCD unevenly
 WIDE = [

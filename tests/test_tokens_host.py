@@ -8,6 +8,7 @@ import os
 import pytest
 import torch
 
+from isa_waits import LLVM, functions, short_waits
 from token_refs import attention_ref, norm_ref, rotary_ref
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -148,3 +149,29 @@ def test_frequency_tables():
     f = nnops.rotary_frequencies((2, 4), 16.0, device="cpu")
     assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1.0, 0.25, 1.0, 0.5, 0.25, 0.125]).double())
     assert torch.allclose(nnops.rotary_frequencies((1, 3), 16.0, shared=True, device="cpu"), torch.tensor([1.0, 0.5, 0.25, 0.125]).double())
+
+
+def test_wait_counter():
+    """the way through the branch is the short one; an accumulation chain needs no wait; a filled wait is none too short"""
+    mfma = "v_mfma_f32_32x32x16_bf16 a[0:15], v[0:3], v[4:7], a[0:15]"
+    use = "v_accvgpr_read_b32 v9, a15"
+    long_way = ["v_mov_b32_e32 v20, v21"] * 8
+    (n, want, _, _), = short_waits([mfma, "s_cbranch_vccnz L1"] + long_way + ["L1:", "s_nop 3", use])
+    assert (n, want) == (5, 12)
+    assert not short_waits([mfma, "s_nop 11", "s_cbranch_vccnz L1"] + long_way + ["L1:", use])
+    assert not short_waits([mfma, mfma, "s_nop 7", "s_nop 3", use]) and short_waits([mfma, mfma, "s_nop 7", "s_nop 2", use])
+    assert short_waits(["L0:", use, mfma, "s_cbranch_scc1 L0", "s_endpgm"])
+    assert short_waits([mfma, "s_nop 2", "v_mfma_f32_32x32x16_bf16 a[16:31], a[0:3], v[4:7], a[16:31]"])
+
+
+@pytest.mark.parametrize("source", ["attention", "attention_bwd"])
+def test_results_of_matrix_instructions_are_waited_for(source, tmp_path):
+    """every way from a product to its use in the built kernels (the values cannot show it: which elements come early depends on the neighbours)"""
+    from sqd import lib
+    obj = os.path.join(lib.OBJ_DIR, source + ".o")
+    if not (os.path.exists(obj) and os.path.exists(LLVM)):
+        pytest.skip("no object file of this source, or no disassembler")
+    code = functions(obj, str(tmp_path))
+    assert sum(any(line.lstrip().startswith("v_mfma") for line in c) for c in code.values()) > 20
+    bad = {name: short_waits(c) for name, c in code.items()}
+    assert not any(bad.values()), {name: b[:2] for name, b in bad.items() if b}
