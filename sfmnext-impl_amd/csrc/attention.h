@@ -289,11 +289,25 @@ __device__ __forceinline__ float half_sum(float v) {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// tanh of a capped score (raw: the product before the scale).  16-bit types: 1 - 2 / (e^{2u} + 1), one exponential and one reciprocal; absolute error
-// 1e-7, i.e. 1e-7 of the cap in the score.  fp32 takes the library's tanh, whose error is relative: with a cap far above the scores the short
-// form would lose them (a cap of 10^4 leaves 6e-4 of a score), and the fp32 products are long enough to hide it.
-template <typename T> __device__ __forceinline__ float tanh_of(float raw, const AttnK &A) {
-    if constexpr (sizeof(T) == 4) return tanhf(raw * A.cap_arg);
+// The forms of a capped score, chosen on the host (cap_form) and compiled apart.  CAP_SHORT: tanh u = 1 - 2 / (e^{2u} + 1), one exponential and one
+// reciprocal, absolute error 4 2^-24, i.e. that times the cap in the score.  Twice that (a score and the row's largest) stays below 2^-14 of a
+// probability, an eighth of half a step of fp16, up to a cap of 128: 16-bit types take it there.  CAP_FULL: the library's tanh, whose error is
+// relative.  fp32 always takes it, and 16-bit types past 128 (a cap of 10^4 leaves 2.4e-3 of a score in the short form, one of 10^8 no score at all).
+enum { CAP_NONE = 0, CAP_SHORT = 1, CAP_FULL = 2 };
+inline int cap_form(float softcap, int dtype) { return softcap == 0.f ? CAP_NONE : dtype != SQD_F32 && softcap <= 128.f ? CAP_SHORT : CAP_FULL; }
+// f(form, bias) as compile-time constants
+template <typename T, typename F> inline void for_scores(int cap, bool bias, F &&f) {
+    auto form = [&](auto c) {
+        if (bias) f(c, std::true_type{});
+        else f(c, std::false_type{});
+    };
+    if (cap == CAP_NONE) form(std::integral_constant<int, CAP_NONE>{});
+    else if (cap == CAP_FULL) form(std::integral_constant<int, CAP_FULL>{});
+    else if constexpr (sizeof(T) == 2) form(std::integral_constant<int, CAP_SHORT>{});
+}
+// tanh of a capped score (raw: the product before the scale)
+template <int CAP> __device__ __forceinline__ float tanh_of(float raw, const AttnK &A) {
+    if constexpr (CAP == CAP_FULL) return tanhf(raw * A.cap_arg);
     else return fmaf(-2.f, __builtin_amdgcn_rcpf(exp2_hw(raw * A.cap_in) + 1.f), 1.f);
 }
 

@@ -46,7 +46,7 @@ template <typename T> __device__ __forceinline__ void store_out(const AttnK &A, 
 }
 
 // The scores of one tile (x: raw products, NB blocks of 32 keys by the wave's 32 rows), the running maximum and sum, and the second product.
-template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
+template <typename T, int DP, int NB, int CAP, bool BIAS> struct Softmax {
     typedef Tile<T, DP> L;
     static constexpr int DB = DP / 32;
     f32x16 o[DB];
@@ -66,7 +66,7 @@ template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    if (CAP) x[nb][r] = tanh_of<T>(x[nb][r], A);
+                    if (CAP) x[nb][r] = tanh_of<CAP>(x[nb][r], A);
                     if (BIAS) x[nb][r] = fmaf(-slope, fabsf(d0 - (float)(nb * 32 + (r & 3) + 8 * (r >> 2))), x[nb][r]);
                 }
         }
@@ -125,7 +125,7 @@ template <typename T, int DP, int NB, bool CAP, bool BIAS> struct Softmax {
     }
 };
 
-template <typename T, int DP, int KT, bool CAP, bool BIAS>
+template <typename T, int DP, int KT, int CAP, bool BIAS>
 __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128 ? 2 : 3) void attn_fwd_kernel(AttnK A) {
     typedef Tile<T, DP> L;
     typedef typename L::frag frag;
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
 // sums and outputs are joined through LDS.  Wave w of split s takes the key tiles s * per + w, + NW, ...
 // Measured: 16 tokens, 32 + 8 heads of 128 bf16, caches of 4351 to 8191 keys (411 MB): 88 us = 4.7 TB/s, and 5 us for the join of the two parts.
 template <typename T, int DP> constexpr int token_waves() { return sizeof(T) == 4 && DP == 128 ? 2 : 4; }       // 64 KB of buffers a wave in fp32
-template <typename T, int DP, int NW, bool CAP, bool BIAS>
+template <typename T, int DP, int NW, int CAP, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
     typedef Tile<T, DP> L;
     typedef typename L::frag frag;
@@ -522,13 +522,7 @@ extern "C" int sqd_attn_fwd(const sqd_attn_args *a) {
                 hipLaunchKernelGGL((attn_fwd_kernel<T, decltype(dp)::value, KT, decltype(cap)::value, decltype(bias)::value>), dim3((unsigned)blocks), dim3(NT),
                                0, st, A);
         };
-        auto flags = [&](auto dp) {
-            const bool cap = a->softcap > 0.f, bias = a->slopes != nullptr;
-            if (cap && bias) go(dp, std::true_type{}, std::true_type{});
-            else if (cap) go(dp, std::true_type{}, std::false_type{});
-            else if (bias) go(dp, std::false_type{}, std::true_type{});
-            else go(dp, std::false_type{}, std::false_type{});
-        };
+        auto flags = [&](auto dp) { for_scores<T>(cap_form(a->softcap, a->dtype), a->slopes != nullptr, [&](auto cap, auto bias) { go(dp, cap, bias); }); };
         switch (pad_dim(a->D)) {
             case 32: flags(std::integral_constant<int, 32>{}); break;
             case 64: flags(std::integral_constant<int, 64>{}); break;

@@ -69,9 +69,9 @@ __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
 }
 
 // probability and score gradient (without the scale) of one pair, e = dP - delta; `see` false: zeros, whatever the products hold
-template <typename T, bool CAP, bool BIAS>
+template <int CAP, bool BIAS>
 __device__ __forceinline__ void pair_grad(float raw, float e, float lse, float slope, float dist, const AttnK &A, bool see, float &p, float &ds) {
-    const float t = CAP ? tanh_of<T>(raw, A) : raw, c = CAP ? A.cap_out : A.scale_log2;
+    const float t = CAP ? tanh_of<CAP>(raw, A) : raw, c = CAP ? A.cap_out : A.scale_log2;
     p = exp2_hw(fmaf(BIAS ? fmaf(-slope, fabsf(dist), t) : t, c, -lse));
     p = see ? p : 0.f;
     const float q = see && p < ONE_LESS ? p : 0.f;
@@ -82,7 +82,7 @@ __device__ __forceinline__ void pair_grad(float raw, float e, float lse, float s
 // KW waves side by side on 32 keys each, times QW on the 32-row parts of a row tile.  A wave needs its gK and gV sums (64 registers each at 128
 // features) and the operands of its keys (32 + 32): with those in registers one wave fits a SIMD and every latency is paid.  KVL keeps the keys'
 // operands in LDS instead: at 128 features 8 waves of 256 registers, two a SIMD; at 64 three workgroups of 4 waves a CU.
-template <typename T, int DP, int KW, int QW, bool KVL, bool CAP, bool BIAS>
+template <typename T, int DP, int KW, int QW, bool KVL, int CAP, bool BIAS>
 __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * sizeof(T) <= 128 ? 2 : 1) void attn_dkv_kernel(AttnK A) {
     constexpr int NT = 64 * KW * QW, QT = 32 * QW, DB = DP / 32;
     typedef Tile<T, DP> L;
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
                 for (int e = 0; e < 4; ++e) {
                     const int r = (2 * H + r2) * 4 + e;
                     const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
-                    pair_grad<T, CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), p[r2 * 4 + e], ds[r2 * 4 + e]);
+                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), p[r2 * 4 + e], ds[r2 * 4 + e]);
                 }
             }
         };
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
         }
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, int CAP, bool BIAS>
 __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_dq_kernel(AttnK A) {
     constexpr int KT = 32, DB = DP / 32;
     typedef Tile<T, DP> L;
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
                     float p;
-                    pair_grad<T, CAP, BIAS>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
+                    pair_grad<CAP, BIAS>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
                 }
             }
         };
@@ -598,7 +598,8 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
         if (p.nk_tiles) attn_doc_ranges(A.k_docs, k_rng, A.B, A.Sk, 1, 32, p.nk_tiles, st);
         auto go = [&](auto dp, auto cap, auto bias) {
             constexpr int DP = decltype(dp)::value;
-            constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
+            constexpr int CAP = decltype(cap)::value;
+            constexpr bool BIAS = decltype(bias)::value;
             if (A.Sk && A.gk) {
                 AttnK K = A;
                 K.ntile = (A.Sk + 32 * p.kw - 1) / (32 * p.kw), K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
@@ -626,13 +627,7 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
                     hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)((p.nq / 4 + NT - 1) / NT)), dim3(NT), 0, st, Q.part_a, (T *)a->gq, p.nq / 4, Q.nsplit);
             }
         };
-        auto flags = [&](auto dp) {
-            const bool cap = a->softcap > 0.f, bias = a->slopes != nullptr;
-            if (cap && bias) go(dp, std::true_type{}, std::true_type{});
-            else if (cap) go(dp, std::true_type{}, std::false_type{});
-            else if (bias) go(dp, std::false_type{}, std::true_type{});
-            else go(dp, std::false_type{}, std::false_type{});
-        };
+        auto flags = [&](auto dp) { for_scores<T>(cap_form(a->softcap, a->dtype), a->slopes != nullptr, [&](auto cap, auto bias) { go(dp, cap, bias); }); };
         if (a->D <= 32) flags(std::integral_constant<int, 32>{});
         else if (a->D <= 64) flags(std::integral_constant<int, 64>{});
         else flags(std::integral_constant<int, 128>{});
