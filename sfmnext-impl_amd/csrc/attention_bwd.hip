@@ -75,8 +75,8 @@ __device__ __forceinline__ void pair_grad(float raw, float e, float lse, float s
     p = exp2_hw(fmaf(BIAS ? fmaf(-slope, fabsf(dist), t) : t, c, -lse));
     p = see ? p : 0.f;
     const float q = see && p < ONE_LESS ? p : 0.f;
-    e = see ? e : 0.f;
-    ds = CAP ? q * e * fmaf(-t, t, 1.f) : q * e;
+    if (CAP) e *= fmaf(-t, t, 1.f);                             // (in front of the selection: a hidden pair's t may be NaN)
+    ds = q * (see ? e : 0.f);
 }
 
 // KW waves side by side on 32 keys each, times QW on the 32-row parts of a row tile.  A wave needs its gK and gV sums (64 registers each at 128
@@ -402,7 +402,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     DocWalk walk(A.q_docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, t1);
 
     frag qf[L::KS], gf[L::KS];
-    const bool live = row.lim >= 0;                            // rows that see no key hold anything
+    const int64_t rec = (int64_t)bh * A.rows_padded + R;
+    const bool live = row.on && A.row_lim[rec] >= 0;           // rows that see no key (documents may hide every key of a row's limit) hold anything
     const T *qrow = (const T *)A.q + b * A.qs[0] + (int64_t)row.i * A.qs[1] + (int64_t)(hk * A.G + row.g) * A.qs[2];
     const T *grow = (const T *)A.go + b * A.gos[0] + (int64_t)row.i * A.gos[1] + (int64_t)(hk * A.G + row.g) * A.gos[2];
 #pragma unroll
@@ -411,7 +412,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
         gf[ks] = L::mem_frag(grow, ks, h, A.D, live);
     }
     float lse = INFINITY, delta = 0.f;
-    if (live) lse = A.row_lse[(int64_t)bh * A.rows_padded + R], delta = A.row_delta[(int64_t)bh * A.rows_padded + R];
+    if (live) lse = A.row_lse[rec], delta = A.row_delta[rec];
 
     const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
     const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
