@@ -28,6 +28,7 @@ struct AttnK {
     float *lse, *part_o, *part_lse;
     float *row_lse, *row_delta, *row_pos, *row_slope;  // the backward's copies by packed row, padded to whole tiles (rows_padded a key head)
     int *row_lim, *row_doc;
+    float *lift, *lift_max;                  // fp16 backward: see lifted()
     const float *slopes;
     const int *prefix, *q_docs, *k_docs, *k_len;
     const int2 *doc_rng;                    // per tile of the looped-over side: smallest and largest document id
@@ -310,6 +311,12 @@ template <int CAP> __device__ __forceinline__ float tanh_of(float raw, const Att
     if constexpr (CAP == CAP_FULL) return tanhf(raw * A.cap_arg);
     else return fmaf(-2.f, __builtin_amdgcn_rcpf(exp2_hw(raw * A.cap_in) + 1.f), 1.f);
 }
+
+// fp16 keeps 11 bits down to 2^-14 only, and P and dS of the backward are far smaller: 1 / (keys of a row), times the incoming gradient.  They are
+// packed multiplied by powers of two that the results are divided by in fp32: P by 2^P_LIFT, dS by the largest 2^k that keeps
+// |P (dP - delta)| <= |go_i| |v_j| + |delta_i| below 2^15 for each pair of a batch row's key head (attn_rows_kernel takes the three maxima).
+template <typename T> constexpr bool lifted() { return std::is_same<T, f16_t>::value; }
+constexpr float P_LIFT = 14.f;
 
 // what a row may see: keys j <= lim (lengths, causal order and prefix in one number), document equal
 __device__ __forceinline__ int row_limit(int pos, int len, bool causal, int prefix) { return causal ? min(max(pos, prefix - 1), len - 1) : len - 1; }

@@ -28,18 +28,57 @@ using namespace sqd;
 constexpr int NT = 256, BM = 128;
 constexpr float ONE_LESS = 1.f - 2.384185791015625e-7f;        // 1 - 2^-22
 
+// the larger of a value over the 16 groups of 16 lanes (whose lanes agree); `red` 4 floats, valid in every thread
+__device__ __forceinline__ float group_max(float v, float *red) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    v = fmaxf(v, __shfl_xor(v, 32, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
 // What the two gradient kernels read of a packed row, padded to whole tiles: lse, delta = o.go, the last key it may see (-1: none, and then
 // its q and go are never loaded), document, and with a bias position and slope.  16 lanes a row, 8 features a lane.  o's rounding alone would be
 // as large an error of a gradient as the rounding of dS, so what it left (o_low) is added back.
+// fp16: the largest |go|^2 and |delta| of a workgroup's rows, and in workgroups of their own behind those of the rows the largest |v|^2 of 64
+// keys, one float each (A.lift_max: [key head][go, delta: a float a row workgroup; v: a float a key workgroup]).
+constexpr int VK = 64;
 template <typename T>
 __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
-    const int RT = A.Sq * A.G, c = (threadIdx.x & 15) * 8, hk = blockIdx.y, b = blockIdx.z;
-    const int R = blockIdx.x * (NT / 16) + (threadIdx.x >> 4);
+    __shared__ float red[4];
+    const int RT = A.Sq * A.G, c = (threadIdx.x & 15) * 8, hk = blockIdx.y, b = blockIdx.z, nr = A.rows_padded / (NT / 16);
+    const int64_t bh = (int64_t)b * A.Hkv + hk;
     const int len = A.k_len ? min(max(A.k_len[b], 0), A.Sk) : A.Sk;
+    float *lift_max = lifted<T>() ? A.lift_max + bh * (2 * nr + (A.Sk + VK - 1) / VK) : nullptr;
+    if (lifted<T>() && (int)blockIdx.x >= nr) {
+        const int blk = blockIdx.x - nr;
+        float mx = 0.f;
+#pragma unroll
+        for (int n = 0; n < VK / 16; ++n) {
+            const int j = blk * VK + n * 16 + (threadIdx.x >> 4);
+            const bool on = j < len && (!A.k_docs || A.k_docs[(int64_t)b * A.Sk + j] >= 0);        // the others hold anything
+            float s = 0.f, v[8];
+            if (on && c < A.D) {
+                load_f32<T, 8>((const T *)A.v + b * A.vs[0] + (int64_t)j * A.vs[1] + hk * A.vs[2] + c, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s = fmaf(v[e], v[e], s);
+            }
+#pragma unroll
+            for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 16);
+            mx = fmaxf(mx, s);
+        }
+        mx = group_max(mx, red);
+        if (threadIdx.x == 0) lift_max[2 * nr + blk] = mx;
+        return;
+    }
+    const int R = blockIdx.x * (NT / 16) + (threadIdx.x >> 4);
     const RowOf row = row_of(A, b, R, RT, len, A.prefix ? max(A.prefix[b], 0) : 0);
     const int hq = hk * A.G + row.g;
-    float s = 0.f;
-    if (c < A.D && row.lim >= 0) {
+    const float lse = row.lim >= 0 ? A.lse[bh * RT + R] : INFINITY;
+    const bool live = lse != INFINITY;                         // documents may hide every key of a row that its limit allows
+    float s = 0.f, g2 = 0.f;
+    if (c < A.D && live) {
         const int64_t o = (((int64_t)b * A.Sq + row.i) * A.Hq + hq) * A.D + c;
         float u[8], v[8];
         load_f32<T, 8>((const T *)A.o + o, u);
@@ -51,30 +90,64 @@ __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
         load_f32<T, 8>((const T *)A.go + b * A.gos[0] + (int64_t)row.i * A.gos[1] + hq * A.gos[2] + c, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s = fmaf(u[e], v[e], s);
+        if (lifted<T>())
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g2 = fmaf(v[e], v[e], g2);
     }
 #pragma unroll
-    for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 16);
+    for (int k = 8; k > 0; k >>= 1) {
+        s += __shfl_xor(s, k, 16);
+        if (lifted<T>()) g2 += __shfl_xor(g2, k, 16);
+    }
     if ((threadIdx.x & 15) == 0) {
-        const int64_t bh = (int64_t)b * A.Hkv + hk, at = bh * A.rows_padded + R;
-        const float lse = row.lim >= 0 ? A.lse[bh * RT + R] : INFINITY;
+        const int64_t at = bh * A.rows_padded + R;
         A.row_delta[at] = s;
-        A.row_lse[at] = lse;
-        A.row_lim[at] = lse == INFINITY ? -1 : row.lim;        // documents may hide every key of a row that its limit allows
+        A.row_lse[at] = lifted<T>() ? lse - P_LIFT : lse;
+        A.row_lim[at] = live ? row.lim : -1;
         A.row_doc[at] = row.qd;
         if (A.slopes) {
             A.row_pos[at] = (float)row.pos;
             A.row_slope[at] = A.slopes[hq] * A.unit_inv;
         }
     }
+    if (lifted<T>()) {
+        const float gm = group_max(g2, red), dm = group_max(fabsf(s), red);
+        if (threadIdx.x == 0) lift_max[blockIdx.x] = gm, lift_max[nr + blockIdx.x] = dm;
+    }
 }
 
-// probability and score gradient (without the scale) of one pair, e = dP - delta; `see` false: zeros, whatever the products hold
-template <int CAP, bool BIAS>
-__device__ __forceinline__ void pair_grad(float raw, float e, float lse, float slope, float dist, const AttnK &A, bool see, float &p, float &ds) {
+// the exponent of dS, one workgroup a key head; a bound that is no number (or no gradient at all) lifts by nothing
+__global__ __launch_bounds__(NT) void attn_lift_kernel(AttnK A) {
+    __shared__ float red[3][4];
+    const int nr = A.rows_padded / (NT / 16), nv = (A.Sk + VK - 1) / VK, tid = threadIdx.x;
+    const float *part = A.lift_max + (int64_t)blockIdx.x * (2 * nr + nv);
+    float mx[3] = {0.f, 0.f, 0.f};
+    for (int i = tid; i < nr; i += NT) mx[0] = fmaxf(mx[0], part[i]), mx[1] = fmaxf(mx[1], part[nr + i]);
+    for (int i = tid; i < nv; i += NT) mx[2] = fmaxf(mx[2], part[2 * nr + i]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) mx[k] = fmaxf(mx[k], __shfl_xor(mx[k], o, 64));
+        if ((tid & 63) == 0) red[k][tid >> 6] = mx[k];
+    }
+    __syncthreads();
+    if (tid) return;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) mx[k] = fmaxf(fmaxf(red[k][0], red[k][1]), fmaxf(red[k][2], red[k][3]));
+    const float bound = sqrtf(mx[0]) * sqrtf(mx[2]) + mx[1];
+    A.lift[blockIdx.x] = bound > 0.f && bound < INFINITY ? (float)min(14 - ilogbf(bound), 64) : 0.f;
+}
+
+// probability and score gradient (without the scale) of one pair, e = dP - delta; `see` false: zeros, whatever the products hold.  p comes lifted
+// as lse is, one_less with it; ds times `factor` on top (LIFT: what the lift of p lacks to that of dS)
+template <int CAP, bool BIAS, bool LIFT>
+__device__ __forceinline__ void pair_grad(float raw, float e, float lse, float slope, float dist, const AttnK &A, bool see, float one_less, float factor, float &p,
+                                          float &ds) {
     const float t = CAP ? tanh_of<CAP>(raw, A) : raw, c = CAP ? A.cap_out : A.scale_log2;
     p = exp2_hw(fmaf(BIAS ? fmaf(-slope, fabsf(dist), t) : t, c, -lse));
     p = see ? p : 0.f;
-    const float q = see && p < ONE_LESS ? p : 0.f;
+    const float q = see && p < one_less ? p : 0.f;
+    if (LIFT) e *= factor;
     if (CAP) e *= fmaf(-t, t, 1.f);                             // (in front of the selection: a hidden pair's t may be NaN)
     ds = q * (see ? e : 0.f);
 }
@@ -144,6 +217,8 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
     DocWalk walk(docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, nt);
     const bool all_on = __all(on);
     const float jf = (float)jl;
+    constexpr float P_UP = lifted<T>() ? 16384.f : 1.f;                            // 2^P_LIFT
+    const float lift = lifted<T>() && RT ? A.lift[bh] : 0.f, factor = ldexpf(1.f, (int)(lift - P_LIFT));
 
     frag kf[KVL ? 1 : L::KS], vf[KVL ? 1 : L::KS];
     const T *kbase = (const T *)A.k + b * A.ks[0] + (int64_t)j0 * A.ks[1] + hk * A.ks[2];
@@ -266,7 +341,8 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
                 for (int e = 0; e < 4; ++e) {
                     const int r = (2 * H + r2) * 4 + e;
                     const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
-                    pair_grad<CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), p[r2 * 4 + e], ds[r2 * 4 + e]);
+                    pair_grad<CAP, BIAS, lifted<T>()>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), ONE_LESS * P_UP, factor,
+                                                      p[r2 * 4 + e], ds[r2 * 4 + e]);
                 }
             }
         };
@@ -341,14 +417,15 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
     }
     if (jl >= A.Sk) return;
     const int64_t o = (((int64_t)b * A.Sk + jl) * A.Hkv + hk) * A.D;
+    const float ku = lifted<T>() ? ldexpf(A.scale, -(int)lift) : A.scale, vu = 1.f / P_UP;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
             const int d = db * 32 + 8 * r4 + 4 * h;
             if (d >= A.D) continue;
-            const float a[4] = {gk[db][4 * r4] * A.scale, gk[db][4 * r4 + 1] * A.scale, gk[db][4 * r4 + 2] * A.scale, gk[db][4 * r4 + 3] * A.scale};
-            const float c[4] = {gv[db][4 * r4], gv[db][4 * r4 + 1], gv[db][4 * r4 + 2], gv[db][4 * r4 + 3]};
+            const float a[4] = {gk[db][4 * r4] * ku, gk[db][4 * r4 + 1] * ku, gk[db][4 * r4 + 2] * ku, gk[db][4 * r4 + 3] * ku};
+            const float c[4] = {gv[db][4 * r4] * vu, gv[db][4 * r4 + 1] * vu, gv[db][4 * r4 + 2] * vu, gv[db][4 * r4 + 3] * vu};
             if (A.nsplit > 1) {
                 const int64_t at = (int64_t)split * A.B * A.Sk * A.Hkv * A.D + o + d;
                 store_f32<float, 4>(A.part_a + at, a);
@@ -413,6 +490,9 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     }
     float lse = INFINITY, delta = 0.f;
     if (live) lse = A.row_lse[rec], delta = A.row_delta[rec];
+    const float lift = lifted<T>() ? A.lift[bh] : 0.f;         // P serves dS alone here: its lift is that of dS
+    if (lifted<T>()) lse += P_LIFT - lift;
+    const float one_less = lifted<T>() ? ldexpf(ONE_LESS, (int)lift) : ONE_LESS;
 
     const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
     const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
@@ -475,7 +555,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
                     float p;
-                    pair_grad<CAP, BIAS>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), p, ds[r]);
+                    pair_grad<CAP, BIAS, false>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), one_less, 1.f, p, ds[r]);
                 }
             }
         };
@@ -500,12 +580,13 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     }
     if (!row.on) return;
     const int64_t out = (((int64_t)b * A.Sq + row.i) * A.Hq + hk * A.G + row.g) * A.D;
+    const float qu = lifted<T>() ? ldexpf(A.scale, -(int)lift) : A.scale;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
             const int d = db * 32 + 8 * r4 + 4 * h;
-            const float v[4] = {gq[db][4 * r4] * A.scale, gq[db][4 * r4 + 1] * A.scale, gq[db][4 * r4 + 2] * A.scale, gq[db][4 * r4 + 3] * A.scale};
+            const float v[4] = {gq[db][4 * r4] * qu, gq[db][4 * r4 + 1] * qu, gq[db][4 * r4 + 2] * qu, gq[db][4 * r4 + 3] * qu};
             if (d >= A.D) continue;
             if (A.nsplit > 1) store_f32<float, 4>(A.part_a + (int64_t)split * A.B * A.Sq * A.Hq * A.D + out + d, v);
             else store_f32<T, 4>((T *)A.gq + out + d, v);
@@ -528,7 +609,7 @@ __global__ __launch_bounds__(NT) void attn_parts_kernel(const float *__restrict_
     store_f32<T, 4>(out + u * 4, a);
 }
 
-struct BwdPlan { int kw, qw, rows_padded, nq_tiles, nk_tiles, k_split, q_split; int64_t rows, nk, nq, parts, scratch; };
+struct BwdPlan { int kw, qw, rows_padded, nq_tiles, nk_tiles, k_split, q_split, nv; int64_t rows, nk, nq, lift, parts, scratch; };
 // parts of the looped-over side: with fewer than 192 workgroups CUs idle, and 512 shorter ones also even out causal rows (168 of fp32, 1281 tokens:
 // dK dV 214 -> 108 us in 3 parts); at least 8 tiles each.  With 240 (3 documents, 3840 tokens) parts lose: 306 -> 493 us, documents being uneven in them.
 int parts_of(int64_t blocks, int64_t tiles) {
@@ -555,7 +636,9 @@ BwdPlan bwd_plan(const sqd_attn_args *a) {
     p.k_split = parts_of((int64_t)((a->Sk + 32 * p.kw - 1) / (32 * p.kw)) * a->B * a->Hkv, (a->Sq * G + QT - 1) / QT);
     p.q_split = parts_of((int64_t)((a->Sq * G + BM - 1) / BM) * a->B * a->Hkv, (a->Sk + 31) / 32);
     const int64_t pk = p.k_split > 1 ? 2 * p.k_split * p.nk : 0, pq = p.q_split > 1 ? p.q_split * p.nq : 0;      // one after the other
-    p.parts = (a->slopes ? 6 : 4) * p.rows + ((int64_t)2 * a->B * (p.nq_tiles + p.nk_tiles) + 3) / 4 * 4;
+    p.nv = a->dtype == SQD_F16 ? (a->Sk + VK - 1) / VK : 0;                        // (fp16: the exponents and the maxima they come from)
+    p.lift = (a->slopes ? 6 : 4) * p.rows + ((int64_t)2 * a->B * (p.nq_tiles + p.nk_tiles) + 3) / 4 * 4;
+    p.parts = p.lift + (a->dtype == SQD_F16 ? ((int64_t)a->B * a->Hkv * (1 + 2 * (p.rows_padded / (NT / 16)) + p.nv) + 3) / 4 * 4 : 0);
     p.scratch = p.parts + (pk > pq ? pk : pq);
     return p;
 }
@@ -591,10 +674,12 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
     A.row_lim = (int *)(a->scratch + 2 * p.rows), A.row_doc = (int *)(a->scratch + 3 * p.rows);
     A.row_pos = a->scratch + 4 * p.rows, A.row_slope = a->scratch + 5 * p.rows;
     int2 *q_rng = reinterpret_cast<int2 *>(a->scratch + (a->slopes ? 6 : 4) * p.rows), *k_rng = q_rng + (int64_t)a->B * p.nq_tiles;
+    A.lift = a->scratch + p.lift, A.lift_max = A.lift + (int64_t)a->B * a->Hkv;
     const hipStream_t st = (hipStream_t)a->stream;
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);
-        if (p.rows) hipLaunchKernelGGL((attn_rows_kernel<T>), dim3(p.rows_padded / 16, A.Hkv, A.B), dim3(NT), 0, st, A);
+        if (p.rows) hipLaunchKernelGGL((attn_rows_kernel<T>), dim3(p.rows_padded / (NT / 16) + p.nv, A.Hkv, A.B), dim3(NT), 0, st, A);
+        if (p.rows && lifted<T>()) hipLaunchKernelGGL(attn_lift_kernel, dim3(A.B * A.Hkv), dim3(NT), 0, st, A);
         if (p.nq_tiles) attn_doc_ranges(A.q_docs, q_rng, A.B, A.Sq, A.G, 32 * p.qw, p.nq_tiles, st);
         if (p.nk_tiles) attn_doc_ranges(A.k_docs, k_rng, A.B, A.Sk, 1, 32, p.nk_tiles, st);
         auto go = [&](auto dp, auto cap, auto bias) {

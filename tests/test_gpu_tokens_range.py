@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+import token_refs
 from token_refs import attention_ref, check
 from test_gpu_tokens import _build, _case, _cuda, _ops
 
@@ -44,3 +45,34 @@ def test_attention_lost_queries_hold_anything_under_every_score(extra, dtype):
     assert not bool(grads[0].cpu()[lost].any())
     for name, got in zip(("gq", "gk", "gv"), grads):
         check(got, ref[name], ref[name + "_tol"], name)
+
+
+# ---------------------------------------------------------------------------------------------- fp16 numbers far below and far above one
+# sizes that reach each gradient kernel: 64 keys by 64 rows (split and whole), 128 keys by 64 rows in 8 waves, 128 keys by 32 rows
+F16_RANGE = [_case(1, 1500, 1500, 1, 1, 64), _case(2, 130, 150, 4, 2, 32, causal=True, softcap=20.0), _case(8, 130, 130, 16, 16, 128, docs=(2, 9)),
+             _case(4, 130, 200, 64, 64, 48, slopes=True)]
+
+
+@pytest.mark.parametrize("size", [3e-5, 1e-4, 1e-3, 1.0, 6e3])
+@pytest.mark.parametrize("n", range(len(F16_RANGE)))
+def test_attention_fp16_gradients_of_any_size(n, size, monkeypatch):
+    """incoming gradients of 3e-5 to 6e3: score gradients keep their 11 bits, however small, and none overflows.  Bounds: those of token_refs.py without
+    the fixed grid of small fp16 numbers inside the sums.  In its place: P has 2^14 of room below that grid (2^-25 - 14 a pair), dS is lifted to
+    within a factor of two of 2^15 / b, b <= 2 max|go| max|v| (2^-25 b / 2^14 a pair); the results' own grid is 2^-25"""
+    c = F16_RANGE[n]
+    # large keys, large gradients of the queries, and the other way round; results have to fit the type
+    for a, b in ((4.0, 0.1), (0.1, 4.0)) if size <= 1 else ((0.1, 0.1),):
+        q, k, v, go, kw = _build(c, F16)
+        q, k, go = (q.float() / 1.5 * a).half(), (k.float() * b).half(), (go.float() * size).half()
+        monkeypatch.setitem(token_refs.HALF_MIN, F16, 0.0)
+        ref = attention_ref(q, k, v, go=go, scale=1.0, **kw)
+        monkeypatch.undo()
+        assert max(float(ref[g].abs().max()) for g in ("gq", "gk", "gv")) < 6e4
+        ds = 2.0 ** -38 * float(go.double().norm(dim=-1).max() * v.double().norm(dim=-1).max())
+        G, over = c["Hq"] // c["Hkv"], lambda t: t.double().abs().sum(1, keepdim=True)                           # noqa: E731
+        heads = lambda t: over(t).view(t.shape[0], 1, c["Hkv"], G, -1).sum(3)                                    # noqa: E731
+        grid = {"gq": ds * over(k).repeat_interleave(G, 2), "gk": ds * heads(q), "gv": 2.0 ** -39 * heads(go)}
+        d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+        o = _ops().attention(*d, scale=1.0, **_cuda(kw))
+        for name, got in zip(("gq", "gk", "gv"), torch.autograd.grad(o, d, go.cuda())):
+            check(got, ref[name], ref[name + "_tol"] + grid[name] + 2.0 ** -25, "%s, %s, %s" % (name, a, b))
