@@ -147,9 +147,8 @@ __device__ __forceinline__ void pair_grad(float raw, float e, float lse, float s
     p = exp2_hw(fmaf(BIAS ? fmaf(-slope, fabsf(dist), t) : t, c, -lse));
     p = see ? p : 0.f;
     const float q = see && p < one_less ? p : 0.f;
-    if (LIFT) e *= factor;
-    if (CAP) e *= fmaf(-t, t, 1.f);                             // (in front of the selection: a hidden pair's t may be NaN)
-    ds = q * (see ? e : 0.f);
+    e = see ? (LIFT ? e * factor : e) : 0.f;
+    ds = CAP ? q * e * fmaf(-t, t, 1.f) : q * e;
 }
 
 // KW waves side by side on 32 keys each, times QW on the 32-row parts of a row tile.  A wave needs its gK and gV sums (64 registers each at 128
