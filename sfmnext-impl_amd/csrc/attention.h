@@ -312,8 +312,8 @@ template <int CAP> __device__ __forceinline__ float tanh_of(float raw, const Att
     else return fmaf(-2.f, __builtin_amdgcn_rcpf(exp2_hw(raw * A.cap_in) + 1.f), 1.f);
 }
 
-// fp16 keeps 11 bits down to 2^-14 only, and P and dS of the backward are far smaller: 1 / (keys of a row), times the incoming gradient.  They are
-// packed multiplied by powers of two that the results are divided by in fp32: P by 2^P_LIFT, dS by the largest 2^k that keeps
+// fp16 keeps 11 bits down to 2^-14 only, and P and dS are far smaller: 1 / (keys of a row), times the incoming gradient.  They are packed multiplied
+// by powers of two that the results are divided by in fp32: P by 2^P_LIFT, dS by the largest 2^k that keeps
 // |P (dP - delta)| <= |go_i| |v_j| + |delta_i| below 2^15 for each pair of a batch row's key head (attn_rows_kernel takes the three maxima).
 template <typename T> constexpr bool lifted() { return std::is_same<T, f16_t>::value; }
 constexpr float P_LIFT = 14.f;

@@ -49,8 +49,11 @@ template <typename T> __device__ __forceinline__ void store_out(const AttnK &A, 
 template <typename T, int DP, int NB, int CAP, bool BIAS> struct Softmax {
     typedef Tile<T, DP> L;
     static constexpr int DB = DP / 32;
+    // fp16: P below 2^-14 of the row's largest would lose bits and below 2^-25 all of them, however many keys there are: it is packed times 2^P_LIFT.
+    // o and l hold that factor, their quotient does not
+    static constexpr float UP = lifted<T>() ? P_LIFT : 0.f;
     f32x16 o[DB];
-    float m, l;
+    float m, l;                             // m + log2(l) - UP: the row's softmax sum
     __device__ __forceinline__ Softmax() : m(-INFINITY), l(0.f) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[db] = f32x16{};
@@ -100,7 +103,7 @@ template <typename T, int DP, int NB, int CAP, bool BIAS> struct Softmax {
                 for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
             m = mn;
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = (m == -INFINITY ? 0.f : m) - UP;
         // 16 keys at a time: their values' operands are read while the step before multiplies, and the exponentials of a step run under its products
         typename L::frag vf[2][DB];
 #pragma unroll
@@ -246,7 +249,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
                 const float v[4] = {sm.o[db][4 * r4] * inv, sm.o[db][4 * r4 + 1] * inv, sm.o[db][4 * r4 + 2] * inv, sm.o[db][4 * r4 + 3] * inv};
                 if (d < A.D) store_f32<float, 4>(po + d, v);
             }
-        if (h == 0) A.part_lse[(int64_t)split * A.B * A.Hkv * RT + at] = l == 0.f ? -INFINITY : sm.m + __builtin_amdgcn_logf(l);
+        if (h == 0) A.part_lse[(int64_t)split * A.B * A.Hkv * RT + at] = l == 0.f ? -INFINITY : sm.m + __builtin_amdgcn_logf(l) - sm.UP;
         return;
     }
     const int64_t out_at = (((int64_t)b * A.Sq + row.i) * A.Hq + hk * A.G + row.g) * A.D;
@@ -258,7 +261,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
             const float v[4] = {sm.o[db][4 * r4] * inv, sm.o[db][4 * r4 + 1] * inv, sm.o[db][4 * r4 + 2] * inv, sm.o[db][4 * r4 + 3] * inv};
             if (d < A.D) store_out<T>(A, out_at + d, v);
         }
-    if (A.lse && h == 0) A.lse[at] = l == 0.f ? INFINITY : sm.m + __builtin_amdgcn_logf(l);
+    if (A.lse && h == 0) A.lse[at] = l == 0.f ? INFINITY : sm.m + __builtin_amdgcn_logf(l) - sm.UP;
 }
 
 // Few rows (Sq G <= 32: one or some tokens against a cache).  Bandwidth bound, so what counts is bytes in flight: every wave takes 32 keys of its
@@ -378,8 +381,8 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
         }
     }
     if (tid < RT) {                                             // tid < 32: lane = row
-        if (A.nsplit > 1) A.part_lse[(int64_t)split * rows + at0 + R] = sum == 0.f ? -INFINITY : mx + __builtin_amdgcn_logf(sum);
-        else if (A.lse) A.lse[at0 + R] = sum == 0.f ? INFINITY : mx + __builtin_amdgcn_logf(sum);
+        if (A.nsplit > 1) A.part_lse[(int64_t)split * rows + at0 + R] = sum == 0.f ? -INFINITY : mx + __builtin_amdgcn_logf(sum) - sm.UP;
+        else if (A.lse) A.lse[at0 + R] = sum == 0.f ? INFINITY : mx + __builtin_amdgcn_logf(sum) - sm.UP;
     }
 }
 

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import token_refs
-from token_refs import attention_ref, check
+from token_refs import HALF, attention_ref, check
 from test_gpu_tokens import _build, _case, _cuda, _ops
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +76,18 @@ def test_attention_fp16_gradients_of_any_size(n, size, monkeypatch):
         o = _ops().attention(*d, scale=1.0, **_cuda(kw))
         for name, got in zip(("gq", "gk", "gv"), torch.autograd.grad(o, d, go.cuda())):
             check(got, ref[name], ref[name + "_tol"] + grid[name] + 2.0 ** -25, "%s, %s, %s" % (name, a, b))
+
+
+@pytest.mark.parametrize("Sq", [1, 40])
+def test_attention_fp16_probabilities_far_below_the_largest(Sq):
+    """one key holds nearly all of a row's weight and a value of zero; the output is what 6000 keys of 2^-27 each leave, summed in fp32.  Bound: half a
+    step of the output (2^-11 relative, 2^-25 absolute), half a step of each probability, and the fp32 sums"""
+    S, D = 6000, 16
+    q, k, v = torch.zeros(1, Sq, 1, D), torch.zeros(1, S, 1, D), torch.ones(1, S, 1, D)
+    q[..., 0], k[:, 4321, :, 0], v[:, 4321] = 1.0, 27.0 * math.log(2.0), 0.0
+    q, k, v = q.half(), k.half(), v.half() * 16
+    z = torch.einsum("bihd,bjhd->bij", q.double(), k.double())
+    p = torch.softmax(z, -1)
+    want = torch.einsum("bij,bjhd->bihd", p, v.double())
+    got = _ops().attention(q.cuda(), k.cuda(), v.cuda(), scale=1.0)
+    check(got, want, want.abs() * (2 * HALF[F16] + 2.0 ** -24 * (S + 64)) + 2.0 ** -25, "o")
