@@ -370,6 +370,13 @@ def _index_tensor(who, name, t, shape, device, types):
     return t.contiguous()
 
 
+def _refuse_tangents(who, *tensors):
+    """forward-mode derivatives are not computed: a dual tensor requires no gradient, so without this its tangent would be dropped silently"""
+    fwd = torch.autograd.forward_ad
+    if fwd._current_level >= 0 and any(isinstance(t, torch.Tensor) and fwd.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("sqd: %s: forward-mode derivatives are not supported" % who)
+
+
 def rms_norm_residual(x, weight, residual=None, eps=1e-6):
     """stream = x + residual, kept in the rows' type; y = weight * stream / sqrt(mean(stream^2) + eps) over the last dimension.
     x, residual [..., C] (float32 | bfloat16 | float16), weight [C] in that type or float32 -> (y, stream); residual None: (y, x).
@@ -388,6 +395,7 @@ def rms_norm_residual(x, weight, residual=None, eps=1e-6):
             raise RuntimeError("sqd: %s: residual %s against x %s" % (who, tuple(residual.shape), tuple(x.shape)))
     if not eps >= 0.0:
         raise RuntimeError("sqd: %s: eps = %r" % (who, eps))
+    _refuse_tangents(who, x, weight, residual)
     tokens = _tokens
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         out = tokens.RmsNormResidual.apply(x, weight, residual, float(eps))
@@ -430,6 +438,7 @@ def rotary_axes(q, k, positions, freq, pairs, interleaved=False):
     freq = _index_tensor(who, "freq", freq, (P,), q.device, (torch.float64,))
     if freq.requires_grad:
         raise RuntimeError("sqd: %s: the frequencies are constants; no gradient is computed for them" % who)
+    _refuse_tangents(who, q, k, freq)
     tokens = _tokens
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = tokens.RotaryAxes.apply(q, k, positions, freq, pairs, int(bool(interleaved)))
@@ -478,6 +487,7 @@ def attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefi
         k_docs = _index_tensor(who, "k_docs", k_docs, (B, Sk), q.device, i32)
     if k_len is not None:
         k_len = _index_tensor(who, "k_len", k_len, (B,), q.device, i32)
+    _refuse_tangents(who, q, k, v, slopes)
     tokens = _tokens
     cfg, masks = (scale, softcap, int(bool(causal))), (slopes, prefix, q_docs, k_docs, k_len)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

@@ -91,3 +91,25 @@ def test_attention_fp16_probabilities_far_below_the_largest(Sq):
     want = torch.einsum("bij,bjhd->bihd", p, v.double())
     got = _ops().attention(q.cuda(), k.cuda(), v.cuda(), scale=1.0)
     check(got, want, want.abs() * (2 * HALF[F16] + 2.0 ** -24 * (S + 64)) + 2.0 ** -25, "o")
+
+
+# -------------------------------------------------------------------------------------------------------------- forward-mode derivatives
+def test_forward_mode_derivatives_are_refused():
+    """no tangent is computed, so none may be dropped: with and without other inputs that require a gradient, and in constants"""
+    import torch.autograd.forward_ad as fwd
+    ops = _ops()
+    x, w = torch.randn(4, 8, device="cuda"), torch.ones(8, device="cuda")
+    q = torch.randn(1, 4, 2, 16, device="cuda")
+    pos, freq, slopes = torch.zeros(4, 1, device="cuda", dtype=torch.int32), torch.zeros(8, device="cuda", dtype=torch.float64), torch.ones(2, device="cuda")
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))                                                    # noqa: E731
+        calls = [lambda: ops.rms_norm_residual(dual(x), w), lambda: ops.rms_norm_residual(x, dual(w)), lambda: ops.rms_norm_residual(x, w, dual(x)),
+                 lambda: ops.rotary_axes(dual(q), q, pos, freq, (8,)), lambda: ops.rotary_axes(q, dual(q), pos, freq, (8,)), lambda: ops.rotary_axes(q, None, pos, dual(freq), (8,)),
+                 lambda: ops.attention(dual(q), q, q), lambda: ops.attention(q, dual(q), q), lambda: ops.attention(q, q, dual(q)), lambda: ops.attention(q, q, q, slopes=dual(slopes)),
+                 lambda: ops.attention(dual(q), q.clone().requires_grad_(True), q), lambda: ops.rms_norm_residual(dual(x), w.clone().requires_grad_(True))]
+        for n, call in enumerate(calls):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="sqd: "):
+                    call()
+                    pytest.fail("call %d was not refused" % n)
+        ops.attention(q, q, q), ops.rms_norm_residual(x, w), ops.rotary_axes(q, q, pos, freq, (8,))     # no tangent: as ever
