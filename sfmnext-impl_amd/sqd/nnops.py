@@ -485,6 +485,8 @@ def attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefi
     if q_docs is not None:
         q_docs = _index_tensor(who, "q_docs", q_docs, (B, Sq), q.device, i32)
         k_docs = _index_tensor(who, "k_docs", k_docs, (B, Sk), q.device, i32)
+        if Sq == 0 or Sk == 0:             # nothing to hide; an empty tensor has no address that could stand for it
+            q_docs = k_docs = None
     if k_len is not None:
         k_len = _index_tensor(who, "k_len", k_len, (B,), q.device, i32)
     _refuse_tangents(who, q, k, v, slopes)

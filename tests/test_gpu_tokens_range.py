@@ -113,3 +113,16 @@ def test_forward_mode_derivatives_are_refused():
                     call()
                     pytest.fail("call %d was not refused" % n)
         ops.attention(q, q, q), ops.rms_norm_residual(x, w), ops.rotary_axes(q, q, pos, freq, (8,))     # no tangent: as ever
+
+
+# --------------------------------------------------------------------------------------------------------------------- empty sides
+@pytest.mark.parametrize("B,Sq,Sk", [(2, 0, 5), (2, 5, 0), (0, 4, 4), (1, 0, 0)])
+def test_attention_empty_sides_with_documents(B, Sq, Sk):
+    z = lambda n: torch.zeros(B, n, 2, 16, device="cuda", requires_grad=True)                                    # noqa: E731
+    docs = [torch.zeros(B, n, device="cuda", dtype=torch.int32) for n in (Sq, Sk)]
+    q, k, v = z(Sq), z(Sk), z(Sk)
+    kw = dict(q_docs=docs[0], k_docs=docs[1], causal=True, prefix=torch.zeros(B, device="cuda", dtype=torch.int32), k_len=torch.full((B,), Sk, device="cuda", dtype=torch.int32))
+    o = _ops().attention(q, k, v, **kw)
+    assert o.shape == q.shape and not bool(o.any())
+    for t, g in zip((q, k, v), torch.autograd.grad(o, (q, k, v), torch.ones_like(o))):
+        assert g.shape == t.shape and not bool(g.any())
