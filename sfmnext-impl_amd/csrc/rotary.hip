@@ -124,7 +124,7 @@ extern "C" int sqd_rotary_axes(const sqd_rotary_args *a) {
     const int64_t BS = (int64_t)a->B * a->S;
     if (BS == 0 || a->Hq + a->Hk == 0) return SQD_OK;
     SQD_CHECK_ARG(a->pos && a->freq && (a->Hq == 0 || (a->q && a->q_out)) && (a->Hk == 0 || (a->k && a->k_out)), "sqd_rotary_axes: null pointer");
-    SQD_CHECK_ARG(a->q != a->q_out && (a->k != a->k_out || !a->k), "sqd_rotary_axes: outputs must not be the inputs");
+    SQD_CHECK_ARG((a->q != a->q_out || !a->q) && (a->k != a->k_out || !a->k), "sqd_rotary_axes: outputs must not be the inputs");
     R.x[0] = a->q, R.x[1] = a->k, R.y[0] = a->q_out, R.y[1] = a->k_out;
     R.heads[0] = a->Hq, R.heads[1] = a->Hk;
     for (int i = 0; i < 3; ++i) {

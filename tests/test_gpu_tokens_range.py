@@ -6,7 +6,7 @@ import torch
 
 import token_refs
 from token_refs import HALF, attention_ref, check
-from test_gpu_tokens import _build, _case, _cuda, _ops
+from test_gpu_tokens import _build, _case, _cuda, _ops, _rand
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -126,3 +126,11 @@ def test_attention_empty_sides_with_documents(B, Sq, Sk):
     assert o.shape == q.shape and not bool(o.any())
     for t, g in zip((q, k, v), torch.autograd.grad(o, (q, k, v), torch.ones_like(o))):
         assert g.shape == t.shape and not bool(g.any())
+
+
+def test_rotary_without_query_heads():
+    g = torch.Generator().manual_seed(4)
+    k = _rand(g, 2, 5, 3, 16, dtype=BF16).cuda()
+    pos, freq = torch.arange(5, device="cuda", dtype=torch.int32)[:, None], _ops().rotary_frequencies((8,))
+    qo, ko = _ops().rotary_axes(k[:, :, :0], k, pos, freq, (8,))
+    assert qo.shape == (2, 5, 0, 16) and torch.equal(ko, _ops().rotary_axes(k, None, pos, freq, (8,))[0])
