@@ -512,7 +512,7 @@ extern "C" int sqd_attn_fwd(const sqd_attn_args *a) {
     SQD_CHECK_ARG(tiles < (1 << 24), "sqd_attn_fwd: too many tokens");
     A.deal = deal(A.B * A.Hkv, (int)tiles);
     const int64_t blocks = p.token ? tiles * A.B * A.Hkv : deal_blocks(A.deal);
-    SQD_CHECK_ARG(blocks < (1ll << 31), "sqd_attn_fwd: too many tokens");
+    SQD_CHECK_ARG(blocks <= max_blocks(NT), "sqd_attn_fwd: too many tokens");
     return for_dtype(a->dtype, [&](auto tt) {
         using T = decltype(tt);
         constexpr int KT = key_tile<T>();

@@ -666,7 +666,11 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
     }
     const BwdPlan p = bwd_plan(a);
     SQD_CHECK_ARG(p.rows < (1 << 28) && a->B < 65536 && a->Hkv < 65536, "%s: too many tokens", who);          // row records: 32-bit offsets between arrays
-    SQD_CHECK_ARG((int64_t)a->B * a->Hkv * 16 * ((a->Sk + 63) / 64 + 8) < (1ll << 31) && p.rows < (1ll << 31), "%s: too many tokens", who);
+    const int nk_wg = (a->Sk + 32 * p.kw - 1) / (32 * p.kw), nq_wg = (int)(((int64_t)a->Sq * (a->Hq / a->Hkv) + BM - 1) / BM);
+    SQD_CHECK_ARG(p.rows_padded / (NT / 16) + p.nv <= max_blocks(NT) && (int64_t)a->B * a->Hkv * (nk_wg + 8) * p.k_split < (1 << 30) &&
+                      (int64_t)a->B * a->Hkv * (nq_wg + 8) * p.q_split < (1 << 30) &&
+                      deal_blocks(deal(a->B * a->Hkv, nk_wg * p.k_split)) <= max_blocks(64 * p.kw * p.qw) &&
+                      deal_blocks(deal(a->B * a->Hkv, nq_wg * p.q_split)) <= max_blocks(NT), "%s: too many tokens", who);
     AttnK A = attn_kargs(a);
     A.rows_padded = p.rows_padded;
     A.row_lse = a->scratch, A.row_delta = a->scratch + p.rows;
@@ -687,7 +691,7 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
             constexpr bool BIAS = decltype(bias)::value;
             if (A.Sk && A.gk) {
                 AttnK K = A;
-                K.ntile = (A.Sk + 32 * p.kw - 1) / (32 * p.kw), K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
+                K.ntile = nk_wg, K.doc_rng = q_rng, K.ndoc_tiles = p.nq_tiles;
                 K.nsplit = p.k_split, K.part_a = a->scratch + p.parts, K.part_b = K.part_a + p.k_split * p.nk;
                 K.deal = deal(A.B * A.Hkv, K.ntile * K.nsplit);
                 const dim3 grid((unsigned)deal_blocks(K.deal));
@@ -704,7 +708,7 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
             }
             if (A.Sq && A.gq) {
                 AttnK Q = A;
-                Q.ntile = (int)(((int64_t)A.Sq * A.G + BM - 1) / BM), Q.doc_rng = k_rng, Q.ndoc_tiles = p.nk_tiles;
+                Q.ntile = nq_wg, Q.doc_rng = k_rng, Q.ndoc_tiles = p.nk_tiles;
                 Q.nsplit = p.q_split, Q.part_a = a->scratch + p.parts;
                 Q.deal = deal(A.B * A.Hkv, Q.ntile * Q.nsplit);
                 hipLaunchKernelGGL((attn_dq_kernel<T, DP, CAP, BIAS>), dim3((unsigned)deal_blocks(Q.deal)), dim3(NT), 0, st, Q);

@@ -26,7 +26,7 @@ struct RotaryArgs {
     const double *freq;                // [P] radians per unit of position
     int axis_end[MAX_AXES];            // pairs below axis_end[a] (and not below axis_end[a-1]) belong to axis a
     int S, D, P, A, tokens;            // tokens per workgroup
-    int64_t BS;
+    int64_t BS, first;                 // first: the launch's first token
     float sign;
 };
 
@@ -34,7 +34,7 @@ template <typename T, typename I, int VEC, bool PAIRED>
 __global__ __launch_bounds__(NT) void rotary_kernel(RotaryArgs R) {
     extern __shared__ float2 cs[];                              // [tokens][P] cos, sin
     __shared__ int64_t src_at[2][MAX_TOKENS];                   // a token's first element in queries / keys
-    const int64_t t0 = (int64_t)blockIdx.x * R.tokens;
+    const int64_t t0 = R.first + (int64_t)blockIdx.x * R.tokens;
     const int nt = (int)min((int64_t)R.tokens, R.BS - t0);
     if (threadIdx.x < 2 * MAX_TOKENS && (int)(threadIdx.x % MAX_TOKENS) < nt) {
         const int w = threadIdx.x / MAX_TOKENS, t = threadIdx.x % MAX_TOKENS;
@@ -120,6 +120,8 @@ extern "C" int sqd_rotary_axes(const sqd_rotary_args *a) {
         P += a->pairs[i];
         R.axis_end[i] = P;
     }
+    // (a token's pieces are counted in 32 bits, one stride past their number)
+    SQD_CHECK_ARG((int64_t)a->Hq * a->D <= (1 << 30) && (int64_t)a->Hk * a->D <= (1 << 30), "sqd_rotary_axes: %d / %d heads of %d features", a->Hq, a->Hk, a->D);
     SQD_CHECK_ARG(P >= 1 && 2 * P <= a->D && a->D % 2 == 0, "sqd_rotary_axes: %d pairs in %d features", P, a->D);
     const int64_t BS = (int64_t)a->B * a->S;
     if (BS == 0 || a->Hq + a->Hk == 0) return SQD_OK;
@@ -135,8 +137,6 @@ extern "C" int sqd_rotary_axes(const sqd_rotary_args *a) {
     R.S = a->S, R.D = a->D, R.P = P, R.A = a->axes, R.BS = BS, R.sign = a->inverse ? -1.f : 1.f;
     // tokens per workgroup: 8 (one round of the trigonometry feeds 8 tokens of traffic), 1 while that leaves CUs without work
     R.tokens = BS >= 8 * 512 ? 8 : 1;
-    const int64_t blocks = (BS + R.tokens - 1) / R.tokens;
-    SQD_CHECK_ARG(blocks < (1ll << 31), "sqd_rotary_axes: %lld tokens", (long long)BS);
     return for_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         constexpr int V = 16 / sizeof(T);
@@ -150,14 +150,17 @@ extern "C" int sqd_rotary_axes(const sqd_rotary_args *a) {
         const size_t lds = (size_t)R.tokens * P * sizeof(float2);
         auto go = [&](auto idx) {
             using I = decltype(idx);
-            const dim3 grid((unsigned)blocks), blk(NT);
+            const dim3 blk(NT);
             const hipStream_t st = (hipStream_t)a->stream;
-            if (a->interleaved) {
-                if (vec) hipLaunchKernelGGL((rotary_kernel<T, I, V, true>), grid, blk, lds, st, R);
-                else hipLaunchKernelGGL((rotary_kernel<T, I, 2, true>), grid, blk, lds, st, R);
-            } else {
-                if (vec) hipLaunchKernelGGL((rotary_kernel<T, I, V, false>), grid, blk, lds, st, R);
-                else hipLaunchKernelGGL((rotary_kernel<T, I, 1, false>), grid, blk, lds, st, R);
+            for (R.first = 0; R.first < BS; R.first += max_blocks(NT) * R.tokens) {
+                const dim3 grid((unsigned)std::min((BS - R.first + R.tokens - 1) / R.tokens, max_blocks(NT)));
+                if (a->interleaved) {
+                    if (vec) hipLaunchKernelGGL((rotary_kernel<T, I, V, true>), grid, blk, lds, st, R);
+                    else hipLaunchKernelGGL((rotary_kernel<T, I, 2, true>), grid, blk, lds, st, R);
+                } else {
+                    if (vec) hipLaunchKernelGGL((rotary_kernel<T, I, V, false>), grid, blk, lds, st, R);
+                    else hipLaunchKernelGGL((rotary_kernel<T, I, 1, false>), grid, blk, lds, st, R);
+                }
             }
             SQD_CHECK_LAUNCH("sqd_rotary_axes");
             return SQD_OK;

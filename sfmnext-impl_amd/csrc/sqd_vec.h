@@ -1,6 +1,8 @@
 // sqd_vec.h — element types of the token operators (token_norm.hip, rotary.hip, attention*.hip): fp32, bf16 and fp16 rows read in 16-byte
 // pieces, all arithmetic in fp32, one round-to-nearest-even at the store.
 #pragma once
+#include <algorithm>
+
 #include "sqd_common.h"
 
 namespace sqd {
@@ -38,6 +40,9 @@ template <typename T, int N> __device__ __forceinline__ void store_f32(T *p, con
     for (int i = 0; i < N; ++i) v.e[i] = from_f32<T>(in[i]);
     *reinterpret_cast<Pack<T, N> *>(p) = v;
 }
+
+// workgroups of NTH threads that one launch takes: a grid counts its threads in 32 bits, and a larger one is cut modulo 2^32 without an error
+constexpr int64_t max_blocks(int nth) { return ((1ll << 32) - 1) / nth; }
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 

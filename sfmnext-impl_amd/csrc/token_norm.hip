@@ -243,7 +243,8 @@ template <typename T, typename F> int for_layout(int C, bool vec_ok, F &&f) {
 }
 
 int check_norm(const char *who, int64_t rows, int C, int dtype, int wdtype) {
-    SQD_CHECK_ARG(rows >= 0 && rows <= (1ll << 30) && C > 0, "%s: bad shape rows=%lld C=%d", who, (long long)rows, C);
+    // (C: column counters run one stride past it, and the weight gradient takes 16 threads a column)
+    SQD_CHECK_ARG(rows >= 0 && rows <= (1ll << 30) && C > 0 && C <= (1 << 27), "%s: bad shape rows=%lld C=%d", who, (long long)rows, C);
     SQD_CHECK_ARG(dtype >= SQD_F32 && dtype <= SQD_F16 && (wdtype == dtype || wdtype == SQD_F32), "%s: element types %d / weight %d unsupported", who, dtype,
                   wdtype);
     return SQD_OK;
@@ -263,12 +264,19 @@ extern "C" int sqd_rms_norm_fwd(const void *x, const void *res, const void *w, v
             const bool vec = C % (16 / sizeof(T)) == 0 && aligned16(x) && aligned16(res) && aligned16(w) && aligned16(y) && aligned16(stream_out);
             return for_layout<T>(C, vec, [&](auto lay) {
                 using L = decltype(lay);
-                if constexpr (L::lanes == 0)
-                    hipLaunchKernelGGL((norm_fwd_any_kernel<T, W>), dim3((unsigned)rows), dim3(NT), 0, (hipStream_t)stream, (const T *)x, (const T *)res,
-                                       (const W *)w, (T *)y, (T *)stream_out, rstd, rows, C, eps);
-                else
-                    hipLaunchKernelGGL((norm_fwd_kernel<T, W, L::lanes, L::vec, L::nc>), dim3((unsigned)((rows * L::lanes + NT - 1) / NT)), dim3(NT), 0,
-                                       (hipStream_t)stream, (const T *)x, (const T *)res, (const W *)w, (T *)y, (T *)stream_out, rstd, rows, C, eps);
+                constexpr int RP = L::lanes ? NT / (L::lanes ? L::lanes : 1) : 1;              // rows of a workgroup
+                for (int64_t r0 = 0; r0 < rows; r0 += max_blocks(NT) * RP) {
+                    const int64_t n = std::min(rows - r0, max_blocks(NT) * RP), o = r0 * C;
+                    const dim3 grid((unsigned)((n + RP - 1) / RP));
+                    const T *xr = (const T *)x + o, *rr = res ? (const T *)res + o : nullptr;
+                    T *yr = (T *)y + o, *sr = stream_out ? (T *)stream_out + o : nullptr;
+                    float *rs = rstd ? rstd + r0 : nullptr;
+                    if constexpr (L::lanes == 0)
+                        hipLaunchKernelGGL((norm_fwd_any_kernel<T, W>), grid, dim3(NT), 0, (hipStream_t)stream, xr, rr, (const W *)w, yr, sr, rs, n, C, eps);
+                    else
+                        hipLaunchKernelGGL((norm_fwd_kernel<T, W, L::lanes, L::vec, L::nc>), grid, dim3(NT), 0, (hipStream_t)stream, xr, rr, (const W *)w, yr,
+                                           sr, rs, n, C, eps);
+                }
                 SQD_CHECK_LAUNCH("sqd_rms_norm_fwd");
                 return SQD_OK;
             });
@@ -294,6 +302,7 @@ extern "C" int sqd_rms_norm_bwd(const void *gy, const void *gs, const void *s, c
             const int rc = for_layout<T>(C, vec, [&](auto lay) {
                 using L = decltype(lay);
                 if constexpr (L::lanes == 0) {
+                    SQD_CHECK_ARG(rows <= max_blocks(NT), "sqd_rms_norm_bwd: %lld rows of %d features", (long long)rows, C);
                     if (rows)
                         hipLaunchKernelGGL((norm_bwd_any_kernel<T, W>), dim3((unsigned)rows), dim3(NT), 0, st, (const T *)gy, (const T *)gs, (const T *)s,
                                            (const W *)w, rstd, (T *)gx, C);

@@ -134,3 +134,30 @@ def test_rotary_without_query_heads():
     pos, freq = torch.arange(5, device="cuda", dtype=torch.int32)[:, None], _ops().rotary_frequencies((8,))
     qo, ko = _ops().rotary_axes(k[:, :, :0], k, pos, freq, (8,))
     assert qo.shape == (2, 5, 0, 16) and torch.equal(ko, _ops().rotary_axes(k, None, pos, freq, (8,))[0])
+
+
+# ----------------------------------------------------------------------------------------------- more threads than a launch can count
+def test_norm_of_more_rows_than_a_launch_counts():
+    """64 threads a row: 2^26 rows are 2^32 threads"""
+    n, C = 2 ** 26 + 5, 8
+    x = torch.full((n, C), 7.0, device="cuda", dtype=BF16)
+    at = torch.tensor([0, 1, 2 ** 20, 2 ** 26 - 5, 2 ** 26 - 4, 2 ** 26 - 1, 2 ** 26, n - 1], device="cuda")
+    x[at] = _rand(torch.Generator().manual_seed(0), len(at), C, dtype=BF16).cuda()
+    x.requires_grad_(True)
+    w = torch.ones(C, device="cuda")
+    y, _ = _ops().rms_norm_residual(x, w, torch.zeros_like(x))
+    few = x.detach()[at].clone().requires_grad_(True)
+    want, _ = _ops().rms_norm_residual(few, w, torch.zeros_like(few))
+    assert torch.equal(y[at], want) and bool((y.detach() == 1.0).sum() >= (n - len(at)) * C)
+    g, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(g[at], torch.autograd.grad(want, few, torch.ones_like(want))[0])
+
+
+def test_rotary_of_more_tokens_than_a_launch_counts():
+    """256 threads for 8 tokens: 2^27 tokens are 2^32 threads"""
+    n = 2 ** 27 + 9
+    q = torch.ones(1, n, 1, 2, device="cuda", dtype=BF16)
+    pos = torch.zeros(n, 1, device="cuda", dtype=torch.int32)
+    pos[-20:] = 1
+    out, _ = _ops().rotary_axes(q, None, pos, torch.full((1,), math.pi / 2, device="cuda", dtype=torch.float64), (1,))
+    assert bool((out[0, :-20] == 1.0).all()) and torch.equal(out[0, -20:, 0].cpu(), torch.tensor([[-1.0, 1.0]] * 20, dtype=BF16))
