@@ -62,6 +62,19 @@ def sources():
 
 
 OBJ_DIR = os.path.join(CSRC, "_build")
+FLAGS_PATH = SO_PATH[:-3] + ".flags"         # what the library and its objects were compiled with: written last, so it never speaks for an unfinished build
+
+
+def compile_flags():
+    """hipcc's flags for every kernel source (tools that compile single files take them from here); SQD_HIPCC_EXTRA: dev knob"""
+    return [f for f in HIPCC_FLAGS if f != "-shared"] + os.environ.get("SQD_HIPCC_EXTRA", "").split()
+
+
+def _other_flags():
+    if not os.path.exists(FLAGS_PATH):
+        return True
+    with open(FLAGS_PATH) as f:
+        return f.read() != "\n".join(compile_flags())
 
 
 def _headers():
@@ -74,11 +87,11 @@ def _obj(src):
 
 def _stale(src, newest_header):
     o = _obj(src)
-    return not os.path.exists(o) or os.path.getmtime(o) < max(os.path.getmtime(src), newest_header)
+    return _other_flags() or not os.path.exists(o) or os.path.getmtime(o) < max(os.path.getmtime(src), newest_header)
 
 
 def needs_build():
-    if not os.path.exists(SO_PATH):
+    if not os.path.exists(SO_PATH) or _other_flags():
         return True
     t = os.path.getmtime(SO_PATH)
     return any(os.path.getmtime(f) > t for f in sources() + _headers())
@@ -86,15 +99,17 @@ def needs_build():
 
 def build(force=False, verbose=False):
     """hipcc cross-compiles every csrc/*.hip for gfx950 (works without a GPU): one object per source file, only the stale
-    ones, in parallel; then one link into sqd/libsqd.so."""
+    ones (older than their sources, or compiled with other flags), in parallel; then one link into sqd/libsqd.so."""
     if not force and not needs_build():
         return SO_PATH
     from concurrent.futures import ThreadPoolExecutor
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     os.makedirs(OBJ_DIR, exist_ok=True)
     newest = max(os.path.getmtime(h) for h in _headers())
-    flags = [f for f in HIPCC_FLAGS if f != "-shared"] + os.environ.get("SQD_HIPCC_EXTRA", "").split()      # (dev knob)
+    flags = compile_flags()
     todo = [s for s in sources() if force or _stale(s, newest)]
+    if os.path.exists(FLAGS_PATH):
+        os.remove(FLAGS_PATH)
 
     def compile_one(src):
         cmd = [hipcc] + flags + ["-c", src, "-o", _obj(src) + ".tmp"]
@@ -113,6 +128,8 @@ def build(force=False, verbose=False):
         print(" ".join(cmd))
     subprocess.check_call(cmd)
     os.replace(SO_PATH + ".tmp", SO_PATH)
+    with open(FLAGS_PATH, "w") as f:
+        f.write("\n".join(flags))
     global _LIB
     _LIB = None
     return SO_PATH

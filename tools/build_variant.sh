@@ -6,7 +6,8 @@ name=$1; file=$2; shift 2
 R=$(cd $(dirname $0)/.. && pwd); B=$R/sfmnext-impl_amd/csrc/_build
 mkdir -p $R/tools/bin
 base=$(basename $file .hip)
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC "$@" -c $R/sfmnext-impl_amd/csrc/$base.hip -o /tmp/variant_${name}_$base.o
+flags=$(PYTHONPATH=$R/sfmnext-impl_amd python3 -c "from sqd import lib; print(*lib.compile_flags())")
+hipcc $flags "$@" -c $R/sfmnext-impl_amd/csrc/$base.hip -o /tmp/variant_${name}_$base.o
 objs=$(ls $B/*.o | grep -v "/$base.o")
 hipcc --offload-arch=gfx950 -shared -fPIC $objs /tmp/variant_${name}_$base.o -o $R/tools/bin/libsqd_$name.so
 echo built $R/tools/bin/libsqd_$name.so

@@ -5,13 +5,16 @@ usage: python tools/pmc_calib.py        (builds tools/_pmc_calib.so with hipcc i
 import ctypes
 import os
 import subprocess
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
+sys.path.insert(0, os.path.join(os.path.dirname(HERE), "sfmnext-impl_amd"))
 SO = os.path.join(HERE, "_pmc_calib.so")
 
 
 def build():
-    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-shared", os.path.join(HERE, "pmc_calib.hip"), "-o", SO])
+    from sqd import lib
+    subprocess.check_call(["/opt/rocm/bin/hipcc"] + lib.compile_flags() + ["-shared", os.path.join(HERE, "pmc_calib.hip"), "-o", SO])
 
 
 if __name__ == "__main__":
