@@ -228,13 +228,14 @@ __device__ __forceinline__ void product(f32x16 (&acc)[NACC], int D, FA &&frag_a,
         __builtin_amdgcn_sched_barrier(0);
     });
 }
-// The wait from a matrix instruction to the first other use of its result (8 passes: 12 states), written out.  The compiler counts it itself, but where
-// two ways lead to that use, one of them right behind the product, it has counted the longer one: with documents the token kernel then read keys
-// 27 and 31 of a tile before the last step's product was in them.  For such places; the product() of the row kernels is followed by none
-// (tests/test_tokens_host.py looks at every way through the built kernels).
-__device__ __forceinline__ void settle() {
+// The wait from a matrix instruction to the first other use of its result (16 bits: 8 passes, 12 states; fp32: 16 passes, 18 states), written out.  The
+// compiler counts it itself, but where two ways lead to that use, one of them right behind the product, it has counted the longer one: with documents
+// the token kernel then read keys 27 and 31 of a tile before the last step's product was in them.  For such places; the product() of the row kernels
+// is followed by none (tests/test_kernel_waits.py looks at every way through the built kernels).
+template <typename T> __device__ __forceinline__ void settle() {
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 11" ::: "memory");
+    if constexpr (sizeof(T) == 4) asm volatile("s_nop 15\n\ts_nop 1" ::: "memory");
+    else asm volatile("s_nop 11" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
 template <typename T, int KS> constexpr int batch_of() { return sizeof(T) == 4 || KS < 4 ? 2 : 4; }

@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
         f32x16 x[1] = {f32x16{}};
         product<T, 1, L::KS, batch_of<T, L::KS>()>(
             x, A.D, [&](int, int ks) { return L::row_frag(lk, lane & 31, ks, h); }, [&](int ks) { return qf[ks]; });
-        settle();
+        settle<T>();
         const bool part = kdoc != nullptr || __any(row.lim < j0 + 31);
         sm.tile(x, A, lv, ld[wave], kdoc != nullptr, part, j0, row.pos, row.lim, row.qd, slope, lane);
         t += NW;
