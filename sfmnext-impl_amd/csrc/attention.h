@@ -141,8 +141,10 @@ template <typename T, int DP> struct Tile {
 
 // 16 bytes at base + off (this lane's) to LDS byte `lds` + 16 * lane, without a register in between.  The compiler does not see the load:
 // dma_wait() (and a barrier, for other waves' data) comes before the LDS bytes are read.  Lanes switched off leave their 16 bytes as they are.
+// (A base written by a vector instruction would want five states in between, which the compiler does not count into assembly: tests/test_kernel_waits.py
+// looks for one.)
 __device__ __forceinline__ void dma16(const void *base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 // (the builtin and not assembly: the compiler then knows that its own earlier loads have arrived too, and does not wait for them, and with
 // them for a DMA under way, in the middle of a loop)

@@ -47,6 +47,75 @@ def test_the_token_kernel_waits_by_itself(tmp_path):
         assert max(nops) >= (18 if "_kernelIf" in name else 12), (name, max(nops))
 
 
+_SCALAR = re.compile(r"\bs(?:\[(\d+):(\d+)\]|(\d+)\b)")
+
+
+def _scalars(text):
+    out = set()
+    for m in _SCALAR.finditer(text):
+        first, last = (m.group(1), m.group(2)) if m.group(1) else (m.group(3), m.group(3))
+        out.update(range(int(first), int(last) + 1))
+    return out | ({"vcc"} if "vcc" in text else set())
+
+
+def short_bases(code):
+    """a scalar register written by a vector instruction and read as the address of a memory access within five states, on any way"""
+    ins, label, found = [], {}, []
+    for line in code:
+        line = line.strip()
+        if line.endswith(":"):
+            label[line[:-1]] = len(ins)
+        elif line:
+            op, _, rest = line.partition(" ")
+            ins.append((op, rest.strip()))
+    for i, (op, rest) in enumerate(ins):
+        dst = _scalars(rest.split(",")[0]) if op.startswith("v_") else set()
+        ways, seen = [(i + 1, 0)] if dst else [], set()
+        while ways:
+            j, n = ways.pop()
+            while j < len(ins) and n < 5 and (j, n) not in seen:
+                seen.add((j, n))
+                o, r = ins[j]
+                if o.startswith(("global_", "buffer_", "flat_")) and _scalars(r) & dst:
+                    found.append((n, op + " " + rest, o + " " + r))
+                    break
+                n += int(r, 0) + 1 if o == "s_nop" else 1
+                if o in ("s_endpgm", "s_setpc_b64"):
+                    break
+                if o == "s_branch":
+                    j = label[r]
+                    continue
+                if o.startswith("s_cbranch"):
+                    ways.append((label[r], n))
+                j += 1
+    return found
+
+
+def test_base_counter():
+    write, load = "v_readfirstlane_b32 s4, v1", "global_load_lds_dwordx4 v2, s[4:5]"
+    assert short_bases([write, "s_mov_b32 m0, s9", "s_nop 0", load]) and not short_bases([write, "s_nop 3", "s_mov_b32 m0, s9", load])
+    assert short_bases([write, "s_cbranch_scc1 L1", "s_nop 4", "L1:", load]) and not short_bases([write, "s_nop 0", "global_load_dword v2, v3, s[6:7]"])
+
+
+@pytest.mark.parametrize("source", ["attention", "attention_bwd"])
+def test_bases_of_loads_in_assembly_are_waited_for(source, tmp_path):
+    bad = {name: short_bases(c) for name, c in _code(source, tmp_path).items()}
+    assert len(bad) > 50 and not any(bad.values()), {name: b[:2] for name, b in bad.items() if b}
+
+
+def test_assembly_that_writes_m0_says_so():
+    """the compiler keeps values of its own there"""
+    from sqd import lib
+    n = 0
+    for src in lib.sources() + lib._headers():
+        with open(src) as f:
+            for block in re.findall(r"asm volatile\(.*?\);", f.read(), re.S):
+                if re.search(r"\bm0,", block):
+                    n += 1
+                    assert '"m0")' in block, (src, block)
+    assert n
+
+
 def test_every_source_with_matrix_instructions_is_looked_at():
     from sqd import lib
     found = set()
