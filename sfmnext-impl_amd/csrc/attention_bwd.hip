@@ -295,8 +295,9 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
     // have the half tile up to the same barrier.
     constexpr bool STAGGER = KW * QW == 8;
     const bool late = STAGGER && qw == 1;
-    auto meet = [] {
+    auto meet = [] {                                           // (this wave's reads of the buffers that the meeting frees have come back)
         asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);                    // lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };

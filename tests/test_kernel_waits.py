@@ -58,9 +58,8 @@ def _scalars(text):
     return out | ({"vcc"} if "vcc" in text else set())
 
 
-def short_bases(code):
-    """a scalar register written by a vector instruction and read as the address of a memory access within five states, on any way"""
-    ins, label, found = [], {}, []
+def _instructions(code):
+    ins, label = [], {}
     for line in code:
         line = line.strip()
         if line.endswith(":"):
@@ -68,6 +67,12 @@ def short_bases(code):
         elif line:
             op, _, rest = line.partition(" ")
             ins.append((op, rest.strip()))
+    return ins, label
+
+
+def short_bases(code):
+    """a scalar register written by a vector instruction and read as the address of a memory access within five states, on any way"""
+    (ins, label), found = _instructions(code), []
     for i, (op, rest) in enumerate(ins):
         dst = _scalars(rest.split(",")[0]) if op.startswith("v_") else set()
         ways, seen = [(i + 1, 0)] if dst else [], set()
@@ -101,6 +106,25 @@ def test_base_counter():
 def test_bases_of_loads_in_assembly_are_waited_for(source, tmp_path):
     bad = {name: short_bases(c) for name, c in _code(source, tmp_path).items()}
     assert len(bad) > 50 and not any(bad.values()), {name: b[:2] for name, b in bad.items() if b}
+
+
+@pytest.mark.parametrize("source", ["attention", "attention_bwd"])
+def test_no_wave_meets_others_with_reads_under_way(source, tmp_path):
+    """behind a barrier another wave overwrites what this one was reading: every read of LDS has come back before it, on every way"""
+    for name, c in _code(source, tmp_path).items():
+        ins, label = _instructions(c)
+        seen, ways = set(), [i + 1 for i, (op, _) in enumerate(ins) if op.startswith("ds_read")]
+        while ways:
+            j = ways.pop()
+            while j < len(ins) and j not in seen:
+                seen.add(j)
+                o, r = ins[j]
+                assert o != "s_barrier", (name, j)
+                if "lgkmcnt(0)" in r or o in ("s_endpgm", "s_setpc_b64"):
+                    break
+                if o.startswith("s_cbranch"):
+                    ways.append(label[r])
+                j = label[r] if o == "s_branch" else j + 1
 
 
 def test_assembly_that_writes_m0_says_so():
