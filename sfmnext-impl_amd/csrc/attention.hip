@@ -289,17 +289,8 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
     const RowOf row = row_of(A, b, R, RT, len, prefix);
     clear_lds<64>(buf[wave], 4 * S::BYTES, lane);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    int kend = len;
-    if (A.causal) kend = max(0, min(len, max(len, prefix)));    // the last query sees every key
-    int dlo = row.qd >= 0 ? row.qd : 0x7fffffff, dhi = row.qd;
-    if (A.q_docs) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            dlo = min(dlo, __shfl_xor(dlo, o, 64));
-            dhi = max(dhi, __shfl_xor(dhi, o, 64));
-        }
-    }
-    const int nt_all = (kend + 31) / 32, per = ((nt_all + A.nsplit - 1) / A.nsplit + NW - 1) / NW * NW;
+    // (causal: the last query sees every key; keys of other documents are hidden pair by pair)
+    const int nt_all = (len + 31) / 32, per = ((nt_all + A.nsplit - 1) / A.nsplit + NW - 1) / NW * NW;
     const int t0 = min(nt_all, split * per), t1 = min(nt_all, t0 + per);
 
     frag qf[L::KS];

@@ -696,11 +696,9 @@ extern "C" int sqd_attn_bwd(const sqd_attn_args *a) {
                 K.nsplit = p.k_split, K.part_a = a->scratch + p.parts, K.part_b = K.part_a + p.k_split * p.nk;
                 K.deal = deal(A.B * A.Hkv, K.ntile * K.nsplit);
                 const dim3 grid((unsigned)deal_blocks(K.deal));
-                if constexpr (sizeof(T) == 2 && DP == 128) {
-                    if (p.kw == 4 && p.qw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 2, true, CAP, BIAS>), grid, dim3(512), 0, st, K);
-                }
                 if (p.kw == 2) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 2, 2, false, CAP, BIAS>), grid, dim3(NT), 0, st, K);
-                else if (p.qw == 1) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 1, (DP * sizeof(T) == 128), CAP, BIAS>), grid, dim3(NT), 0, st, K);
+                else if constexpr (sizeof(T) == 2 && DP == 128) hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 2, true, CAP, BIAS>), grid, dim3(512), 0, st, K);
+                else hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, 1, (DP * sizeof(T) == 128), CAP, BIAS>), grid, dim3(NT), 0, st, K);
                 if (K.nsplit > 1) {                                // (parts of dK, dV are joined before the scratch holds dQ's)
                     const dim3 g2((unsigned)((p.nk / 4 + NT - 1) / NT));
                     hipLaunchKernelGGL((attn_parts_kernel<T>), g2, dim3(NT), 0, st, K.part_a, (T *)a->gk, p.nk / 4, K.nsplit);

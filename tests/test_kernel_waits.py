@@ -127,6 +127,12 @@ def test_no_wave_meets_others_with_reads_under_way(source, tmp_path):
                 j = label[r] if o == "s_branch" else j + 1
 
 
+def test_no_gradient_kernel_is_built_that_no_call_reaches(tmp_path):
+    """16-bit types past 64 features: 128 keys by 64 rows in 8 waves, or 64 keys by 64 rows"""
+    names = [n for n in _code("attention_bwd", tmp_path) if "attn_dkv_kernel" in n]
+    assert any(re.search("bf16_tELi128ELi4ELi2", n) for n in names) and not any(re.search("f16_tELi128ELi4ELi1", n) for n in names)
+
+
 def test_assembly_that_writes_m0_says_so():
     """the compiler keeps values of its own there"""
     from sqd import lib
