@@ -1,0 +1,79 @@
+"""What the 16-bit forward leaves for the backward: o and o_low together are the output to more bits than o has, and delta = (o + o_low) . go needs them.
+Equal scores make every packed probability exactly representable, so that the output's rounding is the only one."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from token_refs import F32 as EPS32
+from token_refs import HALF, check
+
+pytestmark = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+GRID = {BF16: 2.0 ** -134, F16: 2.0 ** -25}
+# many rows; few rows; few rows and many rows whose keys are split over workgroups
+SHAPES = [(2, 140, 300, 4, 2, 64), (64, 3, 200, 8, 8, 128), (1, 1, 3000, 4, 1, 128), (1, 200, 2000, 1, 1, 40)]
+
+
+def _uniform(B, Sq, Sk, Hq, Hkv, D, dtype):
+    """equal scores: every key of a head is the same vector"""
+    g = torch.Generator().manual_seed(Sq + Sk)
+    q = torch.randn(B, Sq, Hq, D, generator=g).to(dtype)
+    k = torch.full((B, Sk, Hkv, D), 0.25).to(dtype)
+    v = (2.0 + 0.1 * torch.randn(B, Sk, Hkv, D, generator=g)).to(dtype)
+    go = torch.randn(B, Sq, Hq, D, generator=g).to(dtype)
+    return q, k, v, go
+
+
+def _forward(q, k, v):
+    from sqd import tokens
+    cfg, masks = (q.shape[-1] ** -0.5, 0.0, 0), (None,) * 5
+    return cfg, masks, tokens.attn_fwd(q, k, v, cfg, masks, True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_output_and_what_its_rounding_left(shape, dtype):
+    """o: half a step.  o + o_low: sums of Sk fp32 terms in any order and their quotient, and half a step of o_low, which is half a step of o at most"""
+    q, k, v, _ = _uniform(*shape, dtype)
+    _, _, (o, low, lse) = _forward(q.cuda(), k.cuda(), v.cuda())
+    B, Sq, Sk, Hq, Hkv, D = shape
+    want = v.double().mean(1, keepdim=True).repeat_interleave(Hq // Hkv, 2).expand(B, Sq, Hq, D)
+    fine = want.abs() * (EPS32 * (Sk + 32) + 2 * HALF[dtype] ** 2) + GRID[dtype]
+    check(o, want, fine + want.abs() * HALF[dtype], "o")
+    check(o.double() + low.double(), want, fine, "o + o_low")
+    assert float(low.float().abs().max()) > 0
+    z = torch.einsum("bihd,bhd->bhi", q.double(), k.double()[:, 0].repeat_interleave(Hq // Hkv, 1)) / math.sqrt(D)
+    want_lse = (z / math.log(2.0) + math.log2(Sk)).view(B, Hkv, Hq // Hkv, Sq).transpose(2, 3).reshape(B, Hkv, -1)
+    check(lse, want_lse, EPS32 * ((D + 16) * float(z.abs().max() + 16) + Sk + 64) * torch.ones_like(want_lse), "lse")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[1] > 1])
+def test_gradients_take_what_the_rounding_left(shape, dtype):
+    """the score gradients of a row add up to nothing, and with equal keys so does the queries' gradient: what is left are half steps of dS and fp32 sums.
+    An error of delta comes Sk times instead, and it is half a step of o where o_low is missing: 2^8 or 2^11 times half a step of o_low, 16 times
+    what fp32 adds (a backward that took no notice of o_low would be off by as much either way)"""
+    from sqd import lib, tokens
+    q, k, v, go = _uniform(*shape, dtype)
+    B, Sq, Sk, Hq, Hkv, D = shape
+    d = [t.cuda() for t in (q, k, v)]
+    cfg, masks, (o, low, lse) = _forward(*d)
+    L, dgo = lib.lib(), go.cuda()
+    v64, g64 = v.double().repeat_interleave(Hq // Hkv, 2), go.double()
+    dp = torch.einsum("bihd,bjhd->bhij", g64, v64)
+    ds = (dp - dp.mean(-1, keepdim=True)).abs() / Sk
+    mag = torch.einsum("bihd,bjhd->bhij", g64.abs(), v64.abs()).sum(-1) / Sk                       # what meets in the fp32 sums of a row
+    # half a step of each dS (fp16: lifted clear of its grid); dP, delta and the probabilities in fp32; delta: half a step of o_low
+    row = HALF[dtype] * ds.sum(-1) + EPS32 * (2 * D + Sk + 64) * 2 * mag + 2 * HALF[dtype] ** 2 * mag + GRID[dtype] * g64.abs().sum(-1).transpose(1, 2)
+    tol = D ** -0.5 * 0.25 * row.transpose(1, 2)[..., None].expand(B, Sq, Hq, D) + GRID[dtype]
+    worst = []
+    for left in (low, None):
+        gq, gk, gv = (torch.empty_like(t) for t in d)
+        a = tokens._attn_args(*d, cfg, masks, (o, left, gq, gk, gv, lse, None), dgo)
+        scratch = torch.empty(max(4, L.sqd_attn_bwd_scratch(ctypes.byref(a))), device="cuda")
+        a.scratch = scratch.data_ptr()
+        lib.check(L.sqd_attn_bwd(ctypes.byref(a)), "attn_bwd")
+        worst.append(float((gq.double().cpu().abs() / tol).max()))
+    assert worst[0] <= 1 and worst[1] > 16 * worst[0], worst
