@@ -319,7 +319,7 @@ template <int CAP> __device__ __forceinline__ float tanh_of(float raw, const Att
 // by powers of two that the results are divided by in fp32: P by 2^P_LIFT, dS by the largest 2^k that keeps
 // |P (dP - delta)| <= |go_i| |v_j| + |delta_i| below 2^15 for each pair of a batch row's key head (attn_rows_kernel takes the three maxima).
 template <typename T> constexpr bool lifted() { return std::is_same<T, f16_t>::value; }
-constexpr float P_LIFT = 14.f;
+constexpr float P_LIFT = 14.f, P_SCALE = 16384.f;               // P_SCALE = 2^P_LIFT
 
 // what a row may see: keys j <= lim (lengths, causal order and prefix in one number), document equal
 __device__ __forceinline__ int row_limit(int pos, int len, bool causal, int prefix) { return causal ? min(max(pos, prefix - 1), len - 1) : len - 1; }

@@ -50,10 +50,16 @@ template <typename T, int DP, int NB, int CAP, bool BIAS> struct Softmax {
     typedef Tile<T, DP> L;
     static constexpr int DB = DP / 32;
     // fp16: P below 2^-14 of the row's largest would lose bits and below 2^-25 all of them, however many keys there are: it is packed times 2^P_LIFT.
-    // o and l hold that factor, their quotient does not
-    static constexpr float UP = lifted<T>() ? P_LIFT : 0.f;
+    // o and l hold that factor, their quotient does not.  m is a multiple of 2^-18 then, so that m - P_LIFT is exact (up to 50): lse keeps all its bits,
+    // which the backward's P = 1 of a single key wants
+    static constexpr float UP = lifted<T>() ? P_LIFT : 0.f, DOWN = lifted<T>() ? 1.f / P_SCALE : 1.f;
+    static __device__ __forceinline__ float lse(float m, float l) {
+        const float d = l * DOWN - 1.f;     // next to one, where a single key's sum is, the hardware's logarithm is short of bits
+                                            // (up to 2^-12 the second term, d^2 / 2, is below 2^-25)
+        return m + (lifted<T>() && fabsf(d) < 1.f / 4096.f ? d * 1.44269504f : __builtin_amdgcn_logf(l * DOWN));
+    }
     f32x16 o[DB];
-    float m, l;                             // m + log2(l) - UP: the row's softmax sum
+    float m, l;
     __device__ __forceinline__ Softmax() : m(-INFINITY), l(0.f) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[db] = f32x16{};
@@ -93,7 +99,9 @@ template <typename T, int DP, int NB, int CAP, bool BIAS> struct Softmax {
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[nb][r]);
-        const float mn = fmaxf(m, half_max(mx) * c);
+        mx = half_max(mx) * c;
+        if (lifted<T>()) mx = rintf(mx * 262144.f) * (1.f / 262144.f);
+        const float mn = fmaxf(m, mx);
         if (__builtin_expect(__any(mn > m), 0)) {              // rare once the maximum has settled
             const float alpha = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
             l *= alpha;
@@ -249,7 +257,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
                 const float v[4] = {sm.o[db][4 * r4] * inv, sm.o[db][4 * r4 + 1] * inv, sm.o[db][4 * r4 + 2] * inv, sm.o[db][4 * r4 + 3] * inv};
                 if (d < A.D) store_f32<float, 4>(po + d, v);
             }
-        if (h == 0) A.part_lse[(int64_t)split * A.B * A.Hkv * RT + at] = l == 0.f ? -INFINITY : sm.m + __builtin_amdgcn_logf(l) - sm.UP;
+        if (h == 0) A.part_lse[(int64_t)split * A.B * A.Hkv * RT + at] = l == 0.f ? -INFINITY : sm.lse(sm.m, l);
         return;
     }
     const int64_t out_at = (((int64_t)b * A.Sq + row.i) * A.Hq + hk * A.G + row.g) * A.D;
@@ -261,7 +269,7 @@ __global__ __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128
             const float v[4] = {sm.o[db][4 * r4] * inv, sm.o[db][4 * r4 + 1] * inv, sm.o[db][4 * r4 + 2] * inv, sm.o[db][4 * r4 + 3] * inv};
             if (d < A.D) store_out<T>(A, out_at + d, v);
         }
-    if (A.lse && h == 0) A.lse[at] = l == 0.f ? INFINITY : sm.m + __builtin_amdgcn_logf(l) - sm.UP;
+    if (A.lse && h == 0) A.lse[at] = l == 0.f ? INFINITY : sm.lse(sm.m, l);
 }
 
 // Few rows (Sq G <= 32: one or some tokens against a cache).  Bandwidth bound, so what counts is bytes in flight: every wave takes 32 keys of its
@@ -372,8 +380,8 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnK A) {
         }
     }
     if (tid < RT) {                                             // tid < 32: lane = row
-        if (A.nsplit > 1) A.part_lse[(int64_t)split * rows + at0 + R] = sum == 0.f ? -INFINITY : mx + __builtin_amdgcn_logf(sum) - sm.UP;
-        else if (A.lse) A.lse[at0 + R] = sum == 0.f ? INFINITY : mx + __builtin_amdgcn_logf(sum) - sm.UP;
+        if (A.nsplit > 1) A.part_lse[(int64_t)split * rows + at0 + R] = sum == 0.f ? -INFINITY : sm.lse(mx, sum);
+        else if (A.lse) A.lse[at0 + R] = sum == 0.f ? INFINITY : sm.lse(mx, sum);
     }
 }
 

@@ -10,9 +10,10 @@
 // bias: 46 and 33 us, row records 10 us; 2 x 1281 fp32, 8 + 4 heads of 40, causal, in 3 parts each: 101 and 77 us.  Bound by vector issue (some 12
 // operations and 1 to 3 exponentials or reciprocals a pair) and its overlap with the products.
 //
-// P within 2^-22 of one: every other key's P is below 2^-22 together and dP - delta is the difference of two equal numbers, rounding noise of
-// about that size; dS is taken as zero there (a row that sees ONE key has exactly no gradient for its scores).  P = 0 (masked): dS is zero
-// whatever dP holds.
+// P within 2^-22 of one (fp16, whose lse carries the lift's rounding too: 2^-21): every other key's P is below that together and dP - delta is the
+// difference of two equal numbers, rounding noise of about that size; dS is taken as zero there.  P of a row that sees ONE key is off by half a unit
+// of lse, so such a row has exactly no gradient for its score while |lse| (the score in base 2) is below 8, and noise of (2 D + 64) 2^-24 of
+// sum |go v| beyond.  P = 0 (masked): dS is zero whatever dP holds.
 #include "attention.h"
 
 namespace sqd {
@@ -26,7 +27,7 @@ namespace {
 using namespace sqd;
 
 constexpr int NT = 256, BM = 128;
-constexpr float ONE_LESS = 1.f - 2.384185791015625e-7f;        // 1 - 2^-22
+template <typename T> constexpr float one_less() { return 1.f - (lifted<T>() ? 4.76837158203125e-7f : 2.384185791015625e-7f); }        // 2^-21, 2^-22
 
 // the larger of a value over the 16 groups of 16 lanes (whose lanes agree); `red` 4 floats, valid in every thread
 __device__ __forceinline__ float group_max(float v, float *red) {
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(NT) void attn_rows_kernel(AttnK A) {
     if ((threadIdx.x & 15) == 0) {
         const int64_t at = bh * A.rows_padded + R;
         A.row_delta[at] = s;
-        A.row_lse[at] = lifted<T>() ? lse - P_LIFT : lse;
+        A.row_lse[at] = lse;
         A.row_lim[at] = live ? row.lim : -1;
         A.row_doc[at] = row.qd;
         if (A.slopes) {
@@ -138,16 +139,15 @@ __global__ __launch_bounds__(NT) void attn_lift_kernel(AttnK A) {
     A.lift[blockIdx.x] = bound > 0.f && bound < INFINITY ? (float)min(14 - ilogbf(bound), 64) : 0.f;
 }
 
-// probability and score gradient (without the scale) of one pair, e = dP - delta; `see` false: zeros, whatever the products hold.  p comes lifted
-// as lse is, one_less with it; ds times `factor` on top (LIFT: what the lift of p lacks to that of dS)
-template <int CAP, bool BIAS, bool LIFT>
-__device__ __forceinline__ void pair_grad(float raw, float e, float lse, float slope, float dist, const AttnK &A, bool see, float one_less, float factor, float &p,
-                                          float &ds) {
+// probability and score gradient (without the scale) of one pair, e = dP - delta; `see` false: zeros, whatever the products hold.  fp16: ds
+// comes times `factor` (not by a shift of lse, which would round it)
+template <typename T, int CAP, bool BIAS>
+__device__ __forceinline__ void pair_grad(float raw, float e, float lse, float slope, float dist, const AttnK &A, bool see, float factor, float &p, float &ds) {
     const float t = CAP ? tanh_of<CAP>(raw, A) : raw, c = CAP ? A.cap_out : A.scale_log2;
     p = exp2_hw(fmaf(BIAS ? fmaf(-slope, fabsf(dist), t) : t, c, -lse));
     p = see ? p : 0.f;
-    const float q = see && p < one_less ? p : 0.f;
-    e = see ? (LIFT ? e * factor : e) : 0.f;
+    const float q = see && p < one_less<T>() ? p : 0.f;
+    e = see ? (lifted<T>() ? e * factor : e) : 0.f;
     ds = CAP ? q * e * fmaf(-t, t, 1.f) : q * e;
 }
 
@@ -216,8 +216,8 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
     DocWalk walk(docs ? A.doc_rng + (int64_t)b * A.ndoc_tiles : nullptr, dlo, dhi, nt);
     const bool all_on = __all(on);
     const float jf = (float)jl;
-    constexpr float P_UP = lifted<T>() ? 16384.f : 1.f;                            // 2^P_LIFT
-    const float lift = lifted<T>() && RT ? A.lift[bh] : 0.f, factor = ldexpf(1.f, (int)(lift - P_LIFT));
+    constexpr float P_UP = lifted<T>() ? P_SCALE : 1.f;
+    const float lift = lifted<T>() && RT ? A.lift[bh] : 0.f, factor = ldexpf(1.f, (int)lift);
 
     frag kf[KVL ? 1 : L::KS], vf[KVL ? 1 : L::KS];
     const T *kbase = (const T *)A.k + b * A.ks[0] + (int64_t)j0 * A.ks[1] + hk * A.ks[2];
@@ -341,8 +341,9 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
                 for (int e = 0; e < 4; ++e) {
                     const int r = (2 * H + r2) * 4 + e;
                     const int le = e == 0 ? lim.x : e == 1 ? lim.y : e == 2 ? lim.z : lim.w, de = e == 0 ? qd.x : e == 1 ? qd.y : e == 2 ? qd.z : qd.w;
-                    pair_grad<CAP, BIAS, lifted<T>()>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), ONE_LESS * P_UP, factor,
-                                                      p[r2 * 4 + e], ds[r2 * 4 + e]);
+                    pair_grad<T, CAP, BIAS>(x[r], dp[r], lse[e], sl[e], ps[e] - jf, A, !masked || (jl <= le && de == kd), factor, p[r2 * 4 + e],
+                                                      ds[r2 * 4 + e]);
+                    if (lifted<T>()) p[r2 * 4 + e] *= P_UP;
                 }
             }
         };
@@ -490,9 +491,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
     }
     float lse = INFINITY, delta = 0.f;
     if (live) lse = A.row_lse[rec], delta = A.row_delta[rec];
-    const float lift = lifted<T>() ? A.lift[bh] : 0.f;         // P serves dS alone here: its lift is that of dS
-    if (lifted<T>()) lse += P_LIFT - lift;
-    const float one_less = lifted<T>() ? ldexpf(ONE_LESS, (int)lift) : ONE_LESS;
+    const float lift = lifted<T>() ? A.lift[bh] : 0.f, factor = ldexpf(1.f, (int)lift);
 
     const T *kbase = (const T *)A.k + b * A.ks[0] + hk * A.ks[2], *vbase = (const T *)A.v + b * A.vs[0] + hk * A.vs[2];
     const int *kdoc = A.k_docs ? A.k_docs + (int64_t)b * A.Sk : nullptr;
@@ -555,7 +554,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
                 for (int e = 0; e < 4; ++e) {
                     const int r = r4 * 4 + e, j = j0 + j4 + e, d = e == 0 ? kd.x : e == 1 ? kd.y : e == 2 ? kd.z : kd.w;
                     float p;
-                    pair_grad<CAP, BIAS, false>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), one_less, 1.f, p, ds[r]);
+                    pair_grad<T, CAP, BIAS>(x[r], dp[r], lse, slope, d0 - (float)(8 * r4 + e), A, !masked || (j <= row.lim && d == row.qd), factor, p, ds[r]);
                 }
             }
         };
@@ -610,8 +609,8 @@ __global__ __launch_bounds__(NT) void attn_parts_kernel(const float *__restrict_
 }
 
 struct BwdPlan { int kw, qw, rows_padded, nq_tiles, nk_tiles, k_split, q_split, nv; int64_t rows, nk, nq, lift, parts, scratch; };
-// parts of the looped-over side: with fewer than 192 workgroups CUs idle, and 512 shorter ones also even out causal rows (168 of fp32, 1281 tokens:
-// dK dV 214 -> 108 us in 3 parts); at least 8 tiles each.  With 240 (3 documents, 3840 tokens) parts lose: 306 -> 493 us, documents being uneven in them.
+// parts of the looped-over side (of the whole side, documents or not): with fewer than 192 workgroups CUs idle, and 512 shorter ones also even out
+// causal rows (168 of fp32, 1281 tokens: dK dV 214 -> 108 us in 3 parts); at least 8 tiles each.  With 240 (3 documents, 3840 tokens) parts lose: 306 -> 493 us, documents being uneven in them.
 int parts_of(int64_t blocks, int64_t tiles) {
     int64_t n = blocks && blocks < 192 ? 512 / blocks : 1;
     n = n > tiles / 8 ? tiles / 8 : n;

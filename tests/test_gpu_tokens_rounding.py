@@ -77,3 +77,29 @@ def test_gradients_take_what_the_rounding_left(shape, dtype):
         lib.check(L.sqd_attn_bwd(ctypes.byref(a)), "attn_bwd")
         worst.append(float((gq.double().cpu().abs() / tol).max()))
     assert worst[0] <= 1 and worst[1] > 16 * worst[0], worst
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, F16])
+@pytest.mark.parametrize("std", [0.5, 60.0])
+def test_rows_of_one_key_at_any_score(std, dtype):
+    """single-token documents inside longer rows: no gradient of the score while it is below 8 in base 2; beyond, P is off by half a unit of the score
+    (2^-24 of it, 2^-15 for the scores here) and dP - delta by the roundings of two sums of D products, of o and its quotient"""
+    from sqd import nnops
+    g = torch.Generator().manual_seed(9)
+    B, S, H, D = 2, 150, 2, 128
+    q, k, v, go = (torch.randn(B, S, H, D, generator=g) for _ in range(4))
+    q, k, v, go = (q * std).to(dtype), k.to(dtype), v.to(dtype), go.to(dtype)
+    docs = torch.arange(S, dtype=torch.int32).expand(B, S).contiguous()
+    docs[:, 100:] = 1000                                          # ... and one document of fifty
+    d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    gq, gk, gv = torch.autograd.grad(nnops.attention(*d, q_docs=docs.cuda()), d, go.cuda())
+    noise = D ** -0.5 * EPS32 * (2 * D + 64) * (go.double() * v.double()).abs().sum(-1, keepdim=True) + GRID.get(dtype, 0.0)
+    score = (q.double() * k.double()).sum(-1, keepdim=True).abs() * D ** -0.5 / math.log(2.0)
+    near = score < 7.9
+    assert bool(near[:, :100].any()) and (std < 1 or bool((~near[:, :100]).any()))
+    for got, other in ((gq, k), (gk, q)):
+        got = got.double().cpu()[:, :100]
+        assert not bool(got[near[:, :100].expand_as(got)].any())
+        assert bool((got.abs() <= (noise * other.double().abs())[:, :100] + GRID.get(dtype, 0.0)).all())
+    assert float(score.max()) < 1024 and bool(gq[:, 100:].any())  # (half a unit of a score up to 1024: 2^-15)
+    check(gv[:, :100], go[:, :100].double(), (go.double().abs() * (HALF[dtype] + 2.0 ** -15))[:, :100], "gv")
