@@ -100,7 +100,7 @@ template <typename T, int DP, int NB, int CAP, bool BIAS> struct Softmax {
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[nb][r]);
         mx = half_max(mx) * c;
-        if (lifted<T>()) mx = rintf(mx * 262144.f) * (1.f / 262144.f);
+        if (lifted<T>() && fabsf(mx) < 64.f) mx = rintf(mx * 262144.f) * (1.f / 262144.f);
         const float mn = fmaxf(m, mx);
         if (__builtin_expect(__any(mn > m), 0)) {              // rare once the maximum has settled
             const float alpha = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
