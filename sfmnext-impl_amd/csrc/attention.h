@@ -51,6 +51,12 @@ template <> struct Mma<bf16_t> {
         for (int i = 0; i < 8; ++i) f[i] = (__bf16)p[i];
         return f;
     }
+    static __device__ __forceinline__ frag rest(const float *p, frag hi) {         // what pack left
+        frag f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (__bf16)(p[i] - (float)hi[i]);
+        return f;
+    }
 };
 template <> struct Mma<f16_t> {
     typedef f16x8 frag;
@@ -59,6 +65,12 @@ template <> struct Mma<f16_t> {
         frag f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = (_Float16)p[i];
+        return f;
+    }
+    static __device__ __forceinline__ frag rest(const float *p, frag hi) {
+        frag f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (_Float16)fmaf((float)hi[i], -1.f, p[i]);       // (one instruction; exact)
         return f;
     }
 };

@@ -10,6 +10,10 @@
 // bias: 46 and 33 us, row records 10 us; 2 x 1281 fp32, 8 + 4 heads of 40, causal, in 3 parts each: 101 and 77 us.  Bound by vector issue (some 12
 // operations and 1 to 3 exponentials or reciprocals a pair) and its overlap with the products.
 //
+// Roundings of 16-bit types.  dS is packed in two terms, hi and what hi left (2^-16 and finer of it), and gK and gQ take one product more: with one
+// term its rounding was as large an error as the gradient's own (1.4 to 2 times the error of one rounding together, 1.0 to 1.16 now).  That product
+// and three vector operations a pair cost 12 to 20 % of the two kernels.  P is packed once (gV: 1.4 times one rounding).
+//
 // P within 2^-22 of one (fp16, whose lse carries the lift's rounding too: 2^-21): every other key's P is below that together and dP - delta is the
 // difference of two equal numbers, rounding noise of about that size; dS is taken as zero there.  P of a row that sees ONE key is off by half a unit
 // of lse, so such a row has exactly no gradient for its score while |lse| (the score in base 2) is below 8, and noise of (2 D + 64) 2^-24 of
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
             if (part) pairs(half, std::true_type{});
             else pairs(half, std::false_type{});
         };
-        frag cg[DB], cq[DB], pf, df;
+        frag cg[DB], cq[DB], pf, df, dl;
         auto operands = [&](int row) {
 #pragma unroll
             for (int db = 0; db < DB; ++db) cg[db] = L::col_frag(lg, q0 + row, db, lane);
@@ -363,9 +367,16 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
             for (int db = 0; db < DB; ++db) gv[db] = Mma<T>::mma(cg[db], pf, gv[db]);
 #pragma unroll
             for (int db = 0; db < DB; ++db) gk[db] = Mma<T>::mma(cq[db], df, gk[db]);
+            if constexpr (sizeof(T) == 2)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) gk[db] = Mma<T>::mma(cq[db], dl, gk[db]);
+        };
+        auto packed = [&] {
+            pf = Mma<T>::pack(p), df = Mma<T>::pack(ds);
+            if constexpr (sizeof(T) == 2) dl = Mma<T>::rest(ds, df);
         };
         grads(std::integral_constant<int, 0>{});
-        pf = Mma<T>::pack(p), df = Mma<T>::pack(ds);
+        packed();
         if (STAGGER) {
             if (late) dma_wait();
             meet();
@@ -378,7 +389,7 @@ __global__ __launch_bounds__(64 * KW * QW, KW * QW == 8 ? 2 : KVL ? 3 : DP * siz
         __builtin_amdgcn_sched_barrier(0);
         products();
         grads(std::integral_constant<int, 1>{});
-        pf = Mma<T>::pack(p), df = Mma<T>::pack(ds);
+        packed();
         operands(16);
         __builtin_amdgcn_sched_barrier(0);
         products();
@@ -571,6 +582,11 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_
             const frag df = Mma<T>::pack(&ds[8 * kk]);
 #pragma unroll
             for (int db = 0; db < DB; ++db) gq[db] = Mma<T>::mma(cf[kk][db], df, gq[db]);
+            if constexpr (sizeof(T) == 2) {
+                const frag dl = Mma<T>::rest(&ds[8 * kk], df);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) gq[db] = Mma<T>::mma(cf[kk][db], dl, gq[db]);
+            }
         }
         dma_wait();
         __syncthreads();

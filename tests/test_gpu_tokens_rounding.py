@@ -103,3 +103,22 @@ def test_rows_of_one_key_at_any_score(std, dtype):
         assert bool((got.abs() <= (noise * other.double().abs())[:, :100] + GRID.get(dtype, 0.0)).all())
     assert float(score.max()) < 1024 and bool(gq[:, 100:].any())  # (half a unit of a score up to 1024: 2^-15)
     check(gv[:, :100], go[:, :100].double(), (go.double().abs() * (HALF[dtype] + 2.0 ** -15))[:, :100], "gv")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("kw", [{}, {"causal": True}, {"softcap": 20.0, "causal": True}])
+@pytest.mark.parametrize("B,S,Hq,Hkv,D", [(2, 300, 4, 2, 64), (8, 300, 16, 16, 128), (4, 260, 64, 64, 32)])
+def test_score_gradients_carry_more_than_one_rounding(B, S, Hq, Hkv, D, kw, dtype):
+    """each gradient kernel.  The results' own rounding is one error of relative size r; a second of that size, independent of it, would make 1.41 r (that of dS
+    in one term; the values' gradient has it from P), rounding noise of delta at some hundred keys less than 0.3 r: 1.05 r together"""
+    from sqd import nnops
+    from token_refs import attention_ref
+    g = torch.Generator().manual_seed(S + D)
+    q, k, v, go = (torch.randn(B, S, h, D, generator=g).to(dtype) for h in (Hq, Hkv, Hkv, Hq))
+    d = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(nnops.attention(*d, **kw), d, go.cuda())
+    ref = attention_ref(q, k, v, go=go, **kw)
+    for name, t, most in (("gq", got[0], 1.2), ("gk", got[1], 1.2), ("gv", got[2], 1.5)):
+        once = float((ref[name].to(dtype).double() - ref[name]).norm())
+        err = float((t.double().cpu() - ref[name]).norm())
+        assert err < most * once, (name, err / once)
