@@ -161,3 +161,34 @@ def test_rotary_of_more_tokens_than_a_launch_counts():
     pos[-20:] = 1
     out, _ = _ops().rotary_axes(q, None, pos, torch.full((1,), math.pi / 2, device="cuda", dtype=torch.float64), (1,))
     assert bool((out[0, :-20] == 1.0).all()) and torch.equal(out[0, -20:, 0].cpu(), torch.tensor([[-1.0, 1.0]] * 20, dtype=BF16))
+
+
+# ------------------------------------------------------------------------------------------------------ long caches, fp16 in a captured graph
+@pytest.mark.parametrize("Sq", [2, 40])
+def test_attention_cache_past_32_bit_offsets(Sq):
+    """2.2 million keys of 8 heads of 128: elements past 2^31, bytes past 2^32.  The queries' document is the last hundred keys, whose results and gradients
+    are those of a cache of a hundred; the other keys get none"""
+    S, n, H, D = 2200000, 100, 8, 128
+    c = _case(1, Sq, n, H, H, D, causal=True, slopes=True)
+    q, k, v, go, kw = _build(c, BF16)
+    ref = attention_ref(q, k, v, go=go, **kw)
+    big = []
+    for t in (k, v):
+        b = torch.zeros(1, S, H, D, device="cuda", dtype=BF16)
+        b[:, -n:] = t.cuda()
+        big.append(b.requires_grad_(True))
+    kd = torch.zeros(1, S, device="cuda", dtype=torch.int32)
+    kd[:, -n:] = 7
+    dq = q.cuda().requires_grad_(True)
+    o = _ops().attention(dq, *big, q_docs=torch.full((1, Sq), 7, device="cuda", dtype=torch.int32), k_docs=kd, **_cuda(kw))
+    check(o, ref["o"], ref["o_tol"], "o")
+    gq, gk, gv = torch.autograd.grad(o, [dq] + big, go.cuda())
+    for name, got in (("gq", gq), ("gk", gk[:, -n:]), ("gv", gv[:, -n:])):
+        check(got, ref[name], ref[name + "_tol"], name)
+    assert not bool(gk[:, :-n].any()) and not bool(gv[:, :-n].any())
+
+
+def test_captured_block_replays_in_fp16():
+    """the lifts of the backward are computed on the device, anew in every replay"""
+    import test_gpu_tokens
+    test_gpu_tokens.test_captured_block_replays(F16)
