@@ -769,7 +769,7 @@ int sqd_comm_destroy(sqd_comm *comm);
 #define SQD_BF16 1
 #define SQD_F16 2
 
-/* (20) rows [rows, C], dense.  stream_out = round(x + res) (NULL with res NULL: the rows themselves are normalised),
+/* (20) rows [rows, C], dense, C up to 2^27.  stream_out = round(x + res) (NULL with res NULL: the rows themselves are normalised),
  * y = w * s / sqrt(mean(s^2) + eps) with s = the ROUNDED stream; rstd [rows] (or NULL) is what the backward reads.  w [C] in the rows'
  * type or fp32 (wdtype).
  * bwd: gy, gs (gradient that arrives at the stream, or NULL) -> gx [rows, C] (the gradient of x and of res alike), gw [C] in w's type;
@@ -799,16 +799,19 @@ int sqd_rotary_axes(const sqd_rotary_args *a);
 /* (22) attention.  q [B,Sq,Hq,D]; k, v [B,Sk,Hkv,D], Hq a multiple of Hkv (head h reads key head h / (Hq/Hkv)); element strides of batch,
  * token, head; features dense; pointers and strides 16-byte aligned; D a multiple of 8 up to 128.
  * Strides: tokens below 2^22 elements, heads times their number below 2^28.
- *   z = scale q.k;  softcap c > 0: z = c tanh(z / c);  slopes [Hq] (or NULL): z -= slope |pos_i - j|
+ *   z = scale q.k;  softcap c > 0 (any up to 1e30): z = c tanh(z / c);  slopes [Hq] (or NULL): z -= slope |pos_i - j|
  *   pos_i = i + n - Sq, n = k_len[b] (or NULL: Sk): the queries are the LAST Sq of n positions.  Keys j >= n are hidden.
  *   causal: j <= pos_i is seen; prefix [B] (or NULL; causal only): j < prefix[b] too
  *   q_docs [B,Sq], k_docs [B,Sk] (both or neither): i sees j where the two are equal and >= 0 (negative: padding)
  * A row that sees no key gets zeros, whatever it holds.  Keys j >= n and keys of a negative document are never read.
+ * 16-bit types: the probabilities enter the second product rounded to the type (fp16: times 2^14), the score gradients as two terms of it (fp16:
+ * times the largest power of two that keeps |go| |v| + |o . go| of a key head in range, so incoming gradients may be of any size).
  *   fwd: o [B,Sq,Hq,D] dense; lse [B,Hkv,Sq*G] (G = Hq/Hkv, row i*G + g; log2 of the softmax sum in base-2 scores, +inf for an empty row)
  *        or NULL; o_low (16-bit types, or NULL): what o's rounding left, for the backward.  scratch: sqd_attn_fwd_scratch(a) floats (keys
  *        split over workgroups when there are few rows; 0: none needed).
  *   bwd: q, k, v, o, o_low (or NULL: gradients lose a little), lse as of the forward, go [B,Sq,Hq,D] with its own strides ->
- *        gq [B,Sq,Hq,D] (NULL: not wanted), gk, gv [B,Sk,Hkv,D] (both or neither), dense;  scratch: sqd_attn_bwd_scratch(a) floats.                                                                                    */
+ *        gq [B,Sq,Hq,D] (NULL: not wanted), gk, gv [B,Sk,Hkv,D] (both or neither), dense;  scratch: sqd_attn_bwd_scratch(a) floats.
+ * Row and key tiles beyond what one launch counts (2^24 workgroups) are refused.                                                     */
 typedef struct sqd_attn_args {
     const void *q, *k, *v, *go;
     void *o, *o_low, *gq, *gk, *gv;

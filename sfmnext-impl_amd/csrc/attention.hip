@@ -5,9 +5,11 @@
 // only the key tiles its rows may see: lengths, causal order and prefix end the walk, document ranges skip tiles; the mask itself is applied only in
 // tiles that some row sees in part.
 // Measured (library product of 8192^3 on the same card: 1218 bf16 / 1176 fp16 / 153 fp32 TFLOP/s): 8192 causal fp16 tokens behind a prefix of 1280, 16 + 4
-// heads of 128: 319 .. 327 us = 870 TFLOP/s of what the masks leave; 2 x 3840 bf16 in 3 documents, capped: 133 us = 490 (the cap's exponential and
-// reciprocal are vector work: 0.6 of the cycles, products 0.3); 12 x 480, 12 heads of 64, bf16, distance bias: 32 us; 2 x 1281 fp32, 8 heads of
-// 40, causal: 54 us (fp32 matrix pipe 0.66 busy).  No LDS bank conflicts (counter: 0).
+// heads of 128: 321 .. 327 us = 870 TFLOP/s of what the masks leave, the matrix pipe 0.50 and the vector pipe 0.54 of the time busy; 2 x 3840 bf16 in 3
+// documents, capped: 134 us = 490 (the cap's exponential and reciprocal are vector work: vector 0.56, matrix 0.23); 12 x 480, 12 heads of 64, bf16,
+// distance bias: 32 us (0.51, 0.17); 2 x 1281 fp32, 8 heads of 40, causal: 54 us (matrix 0.64).  The products and the softmax of a wave follow each other,
+// which is what keeps either pipe from being full.  No LDS bank conflicts in the row kernel; the token kernel's join has some (0.31 of its few LDS cycles:
+// rows of 512 bytes).
 #include "attention.h"
 
 namespace {

@@ -6,9 +6,10 @@
 // Two kernels and no atomics, so gradients repeat to the bit: one owns 128 keys and walks the rows that see them (gK, gV: four products of
 // the row tile), one owns 128 rows and walks their keys (gQ: three products).  Recomputing the scores in both costs 7 products where a single kernel
 // with atomic adds into gQ would take 5.
-// Measured: 2 x 3840 bf16 in 3 documents, 16 + 4 heads of 128, capped: gK gV 245 us (530 TFLOP/s), gQ 160 us (610); 12 x 480, 12 heads of 64, distance
-// bias: 46 and 33 us, row records 10 us; 2 x 1281 fp32, 8 + 4 heads of 40, causal, in 3 parts each: 101 and 77 us.  Bound by vector issue (some 12
-// operations and 1 to 3 exponentials or reciprocals a pair) and its overlap with the products.
+// Measured: 2 x 3840 bf16 in 3 documents, 16 + 4 heads of 128, capped: gK gV 278 us (465 TFLOP/s), gQ 186 us (525); 12 x 480, 12 heads of 64, distance
+// bias: 52 and 39 us, row records 10 us; 2 x 1281 fp32, 8 + 4 heads of 40, causal, in 3 parts each: 100 and 76 us.  16 bits: vector pipe 0.38 to 0.55 of
+// the time busy (some 15 operations and 1 to 3 exponentials or reciprocals a pair), matrix pipe 0.25 to 0.34, what does not overlap is waited for.
+// fp32: matrix pipe 0.56 (gK gV) and 0.67 (gQ).  fp16 on top: the exponents of dS, 5 us, and 2 us of row records.
 //
 // Roundings of 16-bit types.  dS is packed in two terms, hi and what hi left (2^-16 and finer of it), and gK and gQ take one product more: with one
 // term its rounding was as large an error as the gradient's own (1.4 to 2 times the error of one rounding together, 1.0 to 1.16 now).  That product
@@ -636,8 +637,8 @@ BwdPlan bwd_plan(const sqd_attn_args *a) {
     BwdPlan p{};
     const int G = a->Hq / a->Hkv;
     // keys and row parts of a workgroup.  128 x 2 with 8 waves where that fits (16-bit types past 64 features) and most CUs get one.  Else 4 waves: 64
-    // x 2 makes twice the workgroups of 128 x 1, which wins once those fill the card by themselves (bf16, 64 features: 576 workgroups of 128 keys
-    // 47 us against 56, 480: 58 against 54; fp32: 768: 482 against 500, 576: 259 against 242)
+    // x 2 makes twice the workgroups of 128 x 1, which wins once those fill the card by themselves (measured with dS in one term, at two sizes a
+    // type: bf16, 64 features: 576 workgroups of 128 keys 47 us against 56, 480: 58 against 54; fp32: 768: 482 against 500, 576: 259 against 242)
     const int64_t wide = (int64_t)((a->Sk + 127) / 128) * a->B * a->Hkv;
     if (a->dtype != SQD_F32 && a->D > 64 && wide >= 192) p.kw = 4, p.qw = 2;
     else if (wide < (a->dtype == SQD_F32 ? 768 : 512)) p.kw = 2, p.qw = 2;

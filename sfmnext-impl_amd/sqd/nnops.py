@@ -380,7 +380,7 @@ def _refuse_tangents(who, *tensors):
 def rms_norm_residual(x, weight, residual=None, eps=1e-6):
     """stream = x + residual, kept in the rows' type; y = weight * stream / sqrt(mean(stream^2) + eps) over the last dimension.
     x, residual [..., C] (float32 | bfloat16 | float16), weight [C] in that type or float32 -> (y, stream); residual None: (y, x).
-    Differentiable in x, residual (the gradients of both outputs join) and weight."""
+    Differentiable in x, residual (the gradients of both outputs join) and weight, once and in reverse mode."""
     who = "rms_norm_residual"
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise RuntimeError("sqd: %s: x must be a tensor [..., C]" % who)
@@ -420,7 +420,7 @@ def rotary_axes(q, k, positions, freq, pairs, interleaved=False):
     """Rotary positions over 1 to 4 axes (time, row, column).  q [B,S,Hq,D], k [B,S,Hk,D] or None; positions [S,A] or [B,S,A] (int32 | int64, any
     sign and size); pairs: for each axis how many of the head's rotation pairs turn with it, P = sum(pairs) <= D / 2 in order; freq [P] float64
     (rotary_frequencies).  Pair p is (p, p + P), interleaved: (2p, 2p + 1); features behind 2P pass unchanged.  -> new dense q, k.
-    Angles are taken in 64 bits.  Differentiable in q and k; freq is a constant (refused if it requires a gradient)."""
+    Angles are taken in 64 bits.  Differentiable in q and k, once and in reverse mode; freq is a constant (refused if it requires a gradient)."""
     who = "rotary_axes"
     _token_tensor(who, "q", q, 4)
     B, S, Hq, D = q.shape
@@ -456,7 +456,11 @@ def attention(q, k, v, scale=None, softcap=0.0, slopes=None, causal=False, prefi
     q_docs [B,Sq], k_docs [B,Sk] (int32; k_docs defaults to q_docs where Sq = Sk): i sees j of its own document; a negative document is padding.
 
     A query that sees no key gets zeros, and zero gradients.  It may hold anything, and so may keys behind n and padding keys.  Elsewhere a masked
-    product is zero times the value, as in any matrix product: infinite or NaN values may reach queries that mask them.  Differentiable in q, k, v; slopes are constants (refused if they require a gradient)."""
+    product is zero times the value, as in any matrix product: infinite or NaN values may reach queries that mask them.
+
+    16-bit types: probabilities are rounded to the type before they meet the values (float16: scaled, so that small ones keep their bits); score
+    gradients enter their products in two terms of the type (float16: scaled by what the incoming gradient and the values allow).
+    Differentiable in q, k, v, once and in reverse mode; slopes are constants (refused if they require a gradient)."""
     who = "attention"
     _token_tensor(who, "q", q, 4), _token_tensor(who, "k", k, 4, q), _token_tensor(who, "v", v, 4, q)
     B, Sq, Hq, D = q.shape

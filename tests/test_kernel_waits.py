@@ -1,29 +1,33 @@
 """Waits that the hardware does not make by itself, along every way through the built kernels of every source (isa_waits.py holds the rules for
 matrix instructions).  An object file that is not there or not up to date is compiled for the test."""
+import functools
 import os
 import re
 import shutil
 import subprocess
+import tempfile
 
 import pytest
 
 from isa_waits import LLVM, functions, short_waits
 
 
-def _code(source, folder):
+@functools.lru_cache(None)
+def _code(source):
     from sqd import lib
     src, obj = os.path.join(lib.CSRC, source + ".hip"), os.path.join(lib.OBJ_DIR, source + ".o")
     if not os.path.exists(LLVM):
         pytest.skip("no disassembler")
-    if lib._stale(src, max(os.path.getmtime(h) for h in lib._headers())):
-        hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
-        if not os.path.exists(hipcc):
-            pytest.skip("no object file of this source, and no compiler")
-        obj = os.path.join(str(folder), source + ".o")
-        subprocess.check_call([hipcc] + lib.compile_flags() + ["-c", src, "-o", obj])
-    out = os.path.join(str(folder), "parts")
-    os.makedirs(out)
-    return functions(obj, out)
+    with tempfile.TemporaryDirectory() as folder:
+        if lib._stale(src, max(os.path.getmtime(h) for h in lib._headers())):
+            hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+            if not os.path.exists(hipcc):
+                pytest.skip("no object file of this source, and no compiler")
+            obj = os.path.join(folder, source + ".o")
+            subprocess.check_call([hipcc] + lib.compile_flags() + ["-c", src, "-o", obj])
+        out = os.path.join(folder, "parts")
+        os.makedirs(out)
+        return functions(obj, out)
 
 
 # sources with matrix instructions; a new one is noticed by the last test
@@ -31,16 +35,16 @@ MATRIX = ["attention", "attention_bwd", "bins", "conv", "sql", "vit"]
 
 
 @pytest.mark.parametrize("source", MATRIX)
-def test_results_of_matrix_instructions_are_waited_for(source, tmp_path):
-    code = _code(source, tmp_path)
+def test_results_of_matrix_instructions_are_waited_for(source):
+    code = _code(source)
     assert any(line.lstrip().startswith("v_mfma") for c in code.values() for line in c)
     bad = {name: short_waits(c) for name, c in code.items()}
     assert not any(bad.values()), {name: b[:2] for name, b in bad.items() if b}
 
 
-def test_the_token_kernel_waits_by_itself(tmp_path):
+def test_the_token_kernel_waits_by_itself():
     """few rows: the product of the scores is followed by a wait of its own, as long as the product's type needs (the compiler's count is not relied on)"""
-    code = {n: c for n, c in _code("attention", tmp_path).items() if "attn_token_kernel" in n}
+    code = {n: c for n, c in _code("attention").items() if "attn_token_kernel" in n}
     assert len(code) > 20
     for name, c in code.items():
         nops = [sum(int(x, 0) + 1 for x in m) for m in (re.findall(r"s_nop (\d+)", "\n".join(c[i:i + 2])) for i in range(len(c)))]
@@ -103,15 +107,15 @@ def test_base_counter():
 
 
 @pytest.mark.parametrize("source", ["attention", "attention_bwd"])
-def test_bases_of_loads_in_assembly_are_waited_for(source, tmp_path):
-    bad = {name: short_bases(c) for name, c in _code(source, tmp_path).items()}
+def test_bases_of_loads_in_assembly_are_waited_for(source):
+    bad = {name: short_bases(c) for name, c in _code(source).items()}
     assert len(bad) > 50 and not any(bad.values()), {name: b[:2] for name, b in bad.items() if b}
 
 
 @pytest.mark.parametrize("source", ["attention", "attention_bwd"])
-def test_no_wave_meets_others_with_reads_under_way(source, tmp_path):
+def test_no_wave_meets_others_with_reads_under_way(source):
     """behind a barrier another wave overwrites what this one was reading: every read of LDS has come back before it, on every way"""
-    for name, c in _code(source, tmp_path).items():
+    for name, c in _code(source).items():
         ins, label = _instructions(c)
         seen, ways = set(), [i + 1 for i, (op, _) in enumerate(ins) if op.startswith("ds_read")]
         while ways:
@@ -127,9 +131,9 @@ def test_no_wave_meets_others_with_reads_under_way(source, tmp_path):
                 j = label[r] if o == "s_branch" else j + 1
 
 
-def test_no_gradient_kernel_is_built_that_no_call_reaches(tmp_path):
+def test_no_gradient_kernel_is_built_that_no_call_reaches():
     """16-bit types past 64 features: 128 keys by 64 rows in 8 waves, or 64 keys by 64 rows"""
-    names = [n for n in _code("attention_bwd", tmp_path) if "attn_dkv_kernel" in n]
+    names = [n for n in _code("attention_bwd") if "attn_dkv_kernel" in n]
     assert any(re.search("bf16_tELi128ELi4ELi2", n) for n in names) and not any(re.search("f16_tELi128ELi4ELi1", n) for n in names)
 
 
