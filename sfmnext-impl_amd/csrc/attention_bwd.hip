@@ -12,7 +12,7 @@
 // fp32: matrix pipe 0.56 (gK gV) and 0.67 (gQ).  fp16 on top: the exponents of dS, 5 us, and 2 us of row records.
 //
 // Roundings of 16-bit types.  dS is packed in two terms, hi and what hi left (2^-16 and finer of it), and gK and gQ take one product more: with one
-// term its rounding was as large an error as the gradient's own (1.4 to 2 times the error of one rounding together, 1.0 to 1.16 now).  That product
+// term its rounding was as large an error as the gradient's own (1.4 to 2 times the error of one rounding together, 1.0 to 1.2 now).  That product
 // and three vector operations a pair cost 12 to 20 % of the two kernels.  P is packed once (gV: 1.4 times one rounding).
 //
 // P within 2^-22 of one (fp16, whose lse carries the lift's rounding too: 2^-21): every other key's P is below that together and dP - delta is the
